@@ -313,6 +313,107 @@ icua_status icua_set_wait_limit(uint32_t polls);
 icua_status icua_dequant(int32_t fmt, int32_t n_rows, int32_t k, const void* packed_dev, float* out_dev,
                          void* stream);
 
+/* ---- paged K/V cache (device pointers, current device) ------------------------------------------
+ * A cache for serving whose memory is handed out in pages: what writes new tokens into it, what
+ * reads it back and the attention of the new tokens over it.  No reference counterpart (its engine
+ * has one contiguous cache per session, Shaders.swift:776-783); head size 128 as everywhere here.
+ *
+ * All pointers in the descriptors are device pointers of the current device, aligned to 16 bytes
+ * (int32 arrays: 4).  The calls only launch on `stream` (a cudaStream_t or NULL): nothing is
+ * allocated, copied or waited for, so they can be captured into a graph.  Lengths and page numbers
+ * are read by the kernels, so a captured call follows what the arrays hold when it is replayed.
+ * Arguments the host can see are checked before anything is launched.  What only the device can see
+ * is checked there: a page number outside [0, n_pages) is left out (not written, read as zeros, its
+ * positions masked) and sets ICUA_FLAG_PAGE; a sequence whose entries contradict each other (cu_q
+ * that descends or passes total_q, a length below 0 or above max_pages * page_size) counts as
+ * without tokens, a token without a position or a rotation row is left out, and both set
+ * ICUA_FLAG_SEQ.  err_dev: optional device int32 that the flags are OR-ed into. */
+enum { ICUA_DT_F32 = 0, ICUA_DT_BF16 = 1, ICUA_DT_F16 = 2 }; /* row types, as icua_gemv's x_dtype */
+/* Third cache type: int8 codes with one fp32 scale per row (position, head): scale = max|x| / 127,
+ * code = x / scale to the nearest even; a row of zeros has the scale 1, a row that holds a NaN or an
+ * infinity reads back as NaN.  Paged caches only (icua_config.kv_dtype stays 16-bit). */
+enum { ICUA_KV_Q8 = 2 };
+enum { ICUA_FLAG_WAIT = 4, ICUA_FLAG_PAGE = 16, ICUA_FLAG_SEQ = 32 };
+
+/* The cache.  Row (page, head, r) is row page * page_rows + head * head_rows + r of both pools, r <
+ * page_size; page_rows = head_rows = 0 means dense pages [page][head][r] (page_rows = n_kv *
+ * page_size, head_rows = page_size).  Other strides (multiples of 16) lay pages over a cache that
+ * exists: an engine-style [head][max_context][128] cache is pages of page_rows = page_size and
+ * head_rows = max_context.  16-bit rows are 256 bytes in the engine's cache order (16-byte chunk c
+ * of position p at place c ^ (p & 7)), q8 rows 128 codes in plain order. */
+typedef struct icua_kv_pages {
+    void* k;            /* pools of rows */
+    void* v;
+    float* k_scale;     /* q8: one scale per row, by row number; else NULL */
+    float* v_scale;
+    int32_t dtype;      /* ICUA_KV_F16, ICUA_KV_BF16 or ICUA_KV_Q8 */
+    int32_t n_kv;       /* kv heads, 1..128 */
+    int32_t page_size;  /* positions per page: 16, 32, 64, 128 or 256 */
+    int32_t n_pages;
+    int64_t page_rows, head_rows;
+} icua_kv_pages;
+
+/* The batch: rows cu_q[s] .. cu_q[s + 1] - 1 of the calls' row arrays are the newest tokens of
+ * sequence s, which has kv_len[s] positions with them: token i of n sits at position kv_len - n + i.
+ * Rows at and behind cu_q[n_seqs] belong to no sequence and stay as they were.  Sequences may share
+ * pages as long as no call writes into a shared one. */
+typedef struct icua_kv_seqs {
+    int32_t n_seqs;            /* 0..1024 */
+    int32_t total_q;           /* rows of the row arrays */
+    int32_t max_q;             /* at least the new tokens of any one sequence */
+    int32_t max_kv;            /* about the longest kv_len: steers the split of the work, nothing else */
+    const int32_t* cu_q;       /* [n_seqs + 1], ascending */
+    const int32_t* kv_len;     /* [n_seqs] */
+    const int32_t* page_table; /* [n_seqs][max_pages]: entries up to a sequence's last page are read */
+    int32_t max_pages;
+} icua_kv_seqs;
+
+/* New tokens on their way into the cache: rows q | k | v of (n_q + 2 n_kv) * 128 elements. */
+typedef struct icua_kv_rows {
+    const void* qkv;
+    int64_t qkv_stride;        /* elements between two tokens' rows, a multiple of 8; 0 = dense */
+    int32_t qkv_dtype;         /* ICUA_DT_* */
+    int32_t n_q;               /* 0..256 */
+    const float* q_norm;       /* [128] RMSNorm weights of every q / k head, or NULL: no norm */
+    const float* k_norm;
+    float eps;
+    const float* rope;         /* [rope_len][64][2] (cos, sin) of the pairs (j, j + 64), or NULL: no rotation */
+    const int32_t* rope_rows;  /* [total_q] table row of each token, or NULL: its position */
+    int32_t rope_len;
+    void* q_out;               /* [total_q][n_q][128] normalised, rotated q, or NULL */
+    int64_t q_stride;          /* elements between two tokens, a multiple of 8; 0 = n_q * 128 */
+    int32_t q_dtype;           /* ICUA_DT_BF16 or ICUA_DT_F16; the cache's type where that is 16-bit */
+} icua_kv_rows;
+/* Per-head RMSNorm and rotate-half rotation of q and k (fp32), q to q_out, k and v into the cache. */
+icua_status icua_kv_write(const icua_kv_pages* pages, const icua_kv_seqs* seqs, const icua_kv_rows* rows,
+                          int32_t* err_dev, void* stream);
+/* The cached rows of the same tokens, dense [total_q][n_kv][128] of type `dtype` (ICUA_DT_*): with
+ * cu_q the sums of the lengths, whole sequences.  k_out or v_out may be NULL. */
+icua_status icua_kv_read(const icua_kv_pages* pages, const icua_kv_seqs* seqs, void* k_out, void* v_out,
+                         int32_t dtype, int32_t* err_dev, void* stream);
+
+typedef struct icua_attn_paged_args {
+    const void* q;             /* [total_q][n_q][128] */
+    void* out;                 /* the same shape; may be q itself */
+    int64_t q_stride, out_stride; /* elements between two tokens, multiples of 8; 0 = n_q * 128 */
+    int32_t dtype;             /* of q and out: ICUA_DT_BF16 or ICUA_DT_F16; the cache's type where that is 16-bit */
+    int32_t n_q;               /* query heads, a multiple of n_kv; head h reads kv head h / (n_q / n_kv) */
+    float scale;               /* of the scores; 0 = 1 / sqrt(128) */
+    void* scratch;             /* device memory for parts of rows, no initialisation needed; calls that can */
+    uint64_t scratch_bytes;    /*   overlap in time need one each */
+} icua_attn_paged_args;
+/* Bytes of scratch that icua_attn_paged needs for these sizes (n_seqs, total_q, max_q; the arrays are
+ * not read); 0 for arguments that it would refuse. */
+uint64_t icua_attn_paged_scratch_bytes(const icua_kv_pages* pages, const icua_kv_seqs* seqs, int32_t n_q);
+/* Causal attention of every new token over its sequence's cache up to its own position (which
+ * icua_kv_write has filled): one token per sequence (decode), drafts, chunks of a prompt and whole
+ * prompts, together in one call.  Scores, softmax and sums in fp32, probabilities rounded to the
+ * type of q.  Rows of a 16-bit cache behind a sequence's end are never used; rows of its own new
+ * tokens must be finite, since a later token's infinity or NaN reaches the earlier ones of the same
+ * call (0 x inf).  A token without a position (kv_len < n) gets zeros. */
+icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs, const icua_attn_paged_args* args,
+                            int32_t* err_dev, void* stream);
+
 /* ---- host quantizers (reference Converter, Convert.swift:208-320) --------------------------- */
 /* q8: codes int8 [rows, cols], scales fp16 bits [rows, cols/32] (Convert.swift:215-241). */
 icua_status icua_quantize_q8(const float* w, int32_t rows, int32_t cols, int8_t* codes, uint16_t* scales);

@@ -12,7 +12,9 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libicua_cud
 
 OK, ERR_INVALID, ERR_CUDA, ERR_OOM, ERR_IO, ERR_FORMAT, ERR_STATE, ERR_CAPACITY, ERR_UNSUPPORTED, ERR_TIMEOUT = range(10)
 FMT_F16, FMT_Q8, FMT_Q4, FMT_Q4S = 0, 1, 2, 3
-KV_F16, KV_BF16 = 0, 1
+KV_F16, KV_BF16, KV_Q8 = 0, 1, 2
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2
+FLAG_WAIT, FLAG_PAGE, FLAG_SEQ = 4, 16, 32
 TID_EMBED, TID_EMBED_SB, TID_FINAL_NORM, TID_LAYER_BASE, TID_PER_LAYER = 315, 316, 317, 318, 14
 SLOT = dict(attn_norm=0, wqkv=1, wqkv_sb=2, q_norm=3, k_norm=4, wo=5, wo_sb=6, mlp_norm=7, wgu=8, wgu_sb=9,
             wd=10, wd_sb=11)
@@ -39,6 +41,30 @@ class IcuaGrammar(C.Structure):
 class IcuaVisual(C.Structure):
     _fields_ = [("pooler", C.POINTER(C.c_float)), ("deepstack", C.POINTER(C.c_float) * 3), ("n_vis", C.c_int32),
                 ("llm_h", C.c_int32), ("llm_w", C.c_int32)]
+
+
+class IcuaKvPages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("dtype", C.c_int32), ("n_kv", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32),
+                ("page_rows", C.c_int64), ("head_rows", C.c_int64)]
+
+
+class IcuaKvSeqs(C.Structure):
+    _fields_ = [("n_seqs", C.c_int32), ("total_q", C.c_int32), ("max_q", C.c_int32), ("max_kv", C.c_int32),
+                ("cu_q", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p), ("max_pages", C.c_int32)]
+
+
+class IcuaKvRows(C.Structure):
+    _fields_ = [("qkv", C.c_void_p), ("qkv_stride", C.c_int64), ("qkv_dtype", C.c_int32), ("n_q", C.c_int32),
+                ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("eps", C.c_float), ("rope", C.c_void_p),
+                ("rope_rows", C.c_void_p), ("rope_len", C.c_int32), ("q_out", C.c_void_p), ("q_stride", C.c_int64),
+                ("q_dtype", C.c_int32)]
+
+
+class IcuaAttnPaged(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("dtype", C.c_int32), ("n_q", C.c_int32), ("scale", C.c_float), ("scratch", C.c_void_p),
+                ("scratch_bytes", C.c_uint64)]
 
 
 class IcuaError(RuntimeError):
@@ -86,6 +112,10 @@ PROTOTYPES = {
     "icua_gemm_q4s": (_I, [_I, _I, _I, _P, _P, _P, _P, _P]),
     "icua_dequant_q4s_f16": (_I, [_I, _I, _P, _P, _P]),
     "icua_gemm_f16": (_I, [_I, _I, _I, _P, _P, _P, _P, _P]),
+    "icua_kv_write": (_I, [C.POINTER(IcuaKvPages), C.POINTER(IcuaKvSeqs), C.POINTER(IcuaKvRows), _P, _P]),
+    "icua_kv_read": (_I, [C.POINTER(IcuaKvPages), C.POINTER(IcuaKvSeqs), _P, _P, _I, _P, _P]),
+    "icua_attn_paged": (_I, [C.POINTER(IcuaKvPages), C.POINTER(IcuaKvSeqs), C.POINTER(IcuaAttnPaged), _P, _P]),
+    "icua_attn_paged_scratch_bytes": (C.c_uint64, [C.POINTER(IcuaKvPages), C.POINTER(IcuaKvSeqs), _I]),
     "icua_dequant": (_I, [_I, _I, _I, _P, _P, _P]),
     "icua_greedy_head_scratch_bytes": (C.c_uint64, [_I]),
     "icua_greedy_head": (_I, [_I, _P, _P, _P, _P, _P, _P, _P]),

@@ -21,7 +21,7 @@ NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-r
               "-Xptxas", "-v"] + ARCH
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-fno-fast-math", "-ffp-contract=off", "-pthread"]
 
-SOURCES_CU = ["engine.cu"]
+SOURCES_CU = ["engine.cu", "paged.cu"]
 SOURCES_CPP = ["pack.cpp"]
 
 
@@ -46,14 +46,19 @@ def build(verbose: bool = False, force: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     objs = []
     log = []
+    # one nvcc per source, side by side
+    running = []
     for src in SOURCES_CU:
         obj = os.path.join(BUILD, src + ".o")
-        cmd = [nvcc()] + NVCC_FLAGS + ["-c", os.path.join(CSRC, src), "-o", obj]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        log.append(r.stdout + r.stderr)
-        if r.returncode != 0:
-            raise RuntimeError("nvcc failed:\n" + r.stdout + r.stderr)
         objs.append(obj)
+        cmd = [nvcc()] + NVCC_FLAGS + ["-c", os.path.join(CSRC, src), "-o", obj]
+        running.append(subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))
+    for p in running:
+        out, _ = p.communicate()
+        log.append(out)
+    for p, out in zip(running, log):
+        if p.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + out)
     for src in SOURCES_CPP:
         obj = os.path.join(BUILD, src + ".o")
         cmd = ["g++"] + CXX_FLAGS + ["-c", os.path.join(CSRC, src), "-o", obj]

@@ -210,6 +210,18 @@ icua_status fail(icua_engine* e, icua_status s, const char* fmt, ...) {
     return s;
 }
 
+}  // namespace
+
+namespace icua_host {
+// Errors of the entry points in other files: the same thread's icua_global_error.
+icua_status set_global_error(icua_status s, const char* msg) {
+    g_error = msg;
+    return s;
+}
+}  // namespace icua_host
+
+namespace {
+
 #define CK(call)                                                                                   \
     do {                                                                                           \
         cudaError_t _e = (call);                                                                   \

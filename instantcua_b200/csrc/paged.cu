@@ -1,0 +1,295 @@
+// Entry points of the paged K/V cache (include/icua.h): argument checks, choice of the kernel
+// variant and launch.  Kernels: paged.cuh (write, read back), paged_attn.cuh (attention).
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+#include <type_traits>
+
+#include "../../include/icua.h"
+#include "paged.cuh"
+#include "paged_attn.cuh"
+
+namespace icua_host {
+icua_status set_global_error(icua_status s, const char* msg);
+}
+
+using namespace icua;
+
+namespace {
+
+icua_status bad(const char* fmt, ...) {
+    char buf[256];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    return icua_host::set_global_error(ICUA_ERR_INVALID, buf);
+}
+
+icua_status cuda_fail(const char* what, cudaError_t e) {
+    char buf[256];
+    snprintf(buf, sizeof buf, "%s: %s", what, cudaGetErrorString(e));
+    return icua_host::set_global_error(ICUA_ERR_CUDA, buf);
+}
+
+bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+// A pointer that the kernels may follow: device (or managed) memory of the current device.
+icua_status check_device_ptr(const void* p, int dev, const char* name) {
+    cudaPointerAttributes a;
+    const cudaError_t e = cudaPointerGetAttributes(&a, p);
+    if (e != cudaSuccess) return cuda_fail("cudaPointerGetAttributes", e);
+    if (a.type == cudaMemoryTypeManaged) return ICUA_OK;
+    if (a.type != cudaMemoryTypeDevice) return bad("%s is not device memory", name);
+    if (a.device != dev) return bad("%s is on device %d, the current device is %d", name, a.device, dev);
+    return ICUA_OK;
+}
+
+icua_status check_cache(const icua_kv_pages* c, const icua_kv_seqs* s, PagesView* P, SeqsView* S) {
+    if (!c || !s) return bad("null argument");
+    if (s->n_seqs < 0 || s->n_seqs > PA_MAX_SEQS || s->total_q < 0 || s->max_q < 0 || s->max_kv < 0 || s->max_pages < 0)
+        return bad("batch sizes out of range (n_seqs 0..%d, the others not negative)", PA_MAX_SEQS);
+    if (c->dtype != ICUA_KV_F16 && c->dtype != ICUA_KV_BF16 && c->dtype != ICUA_KV_Q8) return bad("unknown cache type %d", c->dtype);
+    if (c->n_kv < 1 || c->n_kv > 128) return bad("n_kv %d is not in 1..128", c->n_kv);
+    int sh = 4;
+    while (sh < 8 && (1 << sh) != c->page_size) ++sh;
+    if ((1 << sh) != c->page_size) return bad("page_size %d is not 16, 32, 64, 128 or 256", c->page_size);
+    if (c->n_pages < 0) return bad("n_pages is negative");
+    if (!c->k || !c->v || !aligned(c->k, 16) || !aligned(c->v, 16)) return bad("pools are null or not 16-byte aligned");
+    if (c->dtype == ICUA_KV_Q8 && (!c->k_scale || !c->v_scale || !aligned(c->k_scale, 16) || !aligned(c->v_scale, 16)))
+        return bad("scales of a q8 cache are null or not 16-byte aligned");
+    P->page_rows = c->page_rows;
+    P->head_rows = c->head_rows;
+    if (c->page_rows == 0 && c->head_rows == 0) {
+        P->head_rows = c->page_size;
+        P->page_rows = (int64_t)c->n_kv * c->page_size;
+    }
+    if (P->page_rows < c->page_size || P->page_rows % 16 || P->head_rows < c->page_size || P->head_rows % 16)
+        return bad("page_rows and head_rows are multiples of 16, at least page_size (or both 0)");
+    if (s->n_seqs > 0 && (!s->cu_q || !s->kv_len || (s->max_pages > 0 && !s->page_table))) return bad("null batch arrays");
+    if (!aligned(s->cu_q, 4) || !aligned(s->kv_len, 4) || !aligned(s->page_table, 4)) return bad("batch arrays are not aligned");
+    if ((int64_t)s->max_pages * c->page_size > INT32_MAX) return bad("max_pages * page_size is above 2^31 - 1");
+    P->k = (uint8_t*)c->k;
+    P->v = (uint8_t*)c->v;
+    P->ks = c->k_scale;
+    P->vs = c->v_scale;
+    P->n_kv = c->n_kv;
+    P->ps_shift = sh;
+    P->n_pages = c->n_pages;
+    *S = SeqsView{s->cu_q, s->kv_len, s->page_table, s->n_seqs, s->total_q, s->max_pages};
+    return ICUA_OK;
+}
+
+icua_status current(const icua_kv_pages* c, const void* rows, int* dev) {
+    const cudaError_t e = cudaGetDevice(dev);
+    if (e != cudaSuccess) return cuda_fail("cudaGetDevice", e);
+    icua_status st = check_device_ptr(c->k, *dev, "the K pool");
+    return st != ICUA_OK ? st : check_device_ptr(rows, *dev, "the row array");
+}
+
+constexpr int MAX_DEVICES = 64;
+int sm_count(int dev) {
+    static int n[MAX_DEVICES];
+    if (dev < 0 || dev >= MAX_DEVICES) return 148;
+    if (n[dev] == 0) {
+        int v = 0;
+        n[dev] = cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0 ? v : 148;
+    }
+    return n[dev];
+}
+
+template <auto Kernel>
+cudaError_t allow_smem(int bytes, int dev) {
+    static bool done[MAX_DEVICES];
+    if (dev >= 0 && dev < MAX_DEVICES && done[dev]) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev >= 0 && dev < MAX_DEVICES) done[dev] = true;
+    return e;
+}
+
+// four vectors per half-warp where that still leaves two CTAs (of 16 half-warps) per SM
+int vectors_per_unit(int64_t tokens, int n_vec, int n_sm) { return tokens * ((n_vec + 3) / 4) >= 2ll * 16 * n_sm ? 4 : 1; }
+
+template <typename TI, typename TQ, int KVD>
+cudaError_t launch_write(KvWriteParams& p, int n_sm, cudaStream_t st) {
+    const int n_vec = p.n_q + 2 * p.pages.n_kv;
+    const int vpt = vectors_per_unit(p.seqs.total_q, n_vec, n_sm);
+    p.n_groups = (n_vec + vpt - 1) / vpt;
+    const int64_t grid = ((int64_t)p.seqs.total_q * p.n_groups + 15) / 16;
+    if (vpt == 4) kv_write_kernel<TI, TQ, KVD, 4><<<(unsigned)grid, 256, 0, st>>>(p);
+    else kv_write_kernel<TI, TQ, KVD, 1><<<(unsigned)grid, 256, 0, st>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename TI>
+cudaError_t launch_write_in(KvWriteParams& p, int kvd, int qd, int n_sm, cudaStream_t st) {
+    if (kvd == ICUA_KV_F16) return launch_write<TI, __half, KV_F16>(p, n_sm, st);
+    if (kvd == ICUA_KV_BF16) return launch_write<TI, __nv_bfloat16, KV_BF16>(p, n_sm, st);
+    return qd == ICUA_DT_F16 ? launch_write<TI, __half, KV_Q8>(p, n_sm, st) : launch_write<TI, __nv_bfloat16, KV_Q8>(p, n_sm, st);
+}
+
+template <typename TO, int KVD>
+cudaError_t launch_read_one(KvReadParams& p, int n_sm, cudaStream_t st) {
+    const int n_vec = 2 * p.pages.n_kv;
+    const int vpt = vectors_per_unit(p.seqs.total_q, n_vec, n_sm);
+    p.n_groups = (n_vec + vpt - 1) / vpt;
+    const int64_t grid = ((int64_t)p.seqs.total_q * p.n_groups + 15) / 16;
+    if (vpt == 4) kv_read_kernel<TO, KVD, 4><<<(unsigned)grid, 256, 0, st>>>(p);
+    else kv_read_kernel<TO, KVD, 1><<<(unsigned)grid, 256, 0, st>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename TO>
+cudaError_t launch_read(KvReadParams& p, int kvd, int n_sm, cudaStream_t st) {
+    return kvd == ICUA_KV_F16 ? launch_read_one<TO, KV_F16>(p, n_sm, st)
+         : kvd == ICUA_KV_BF16 ? launch_read_one<TO, KV_BF16>(p, n_sm, st)
+                               : launch_read_one<TO, KV_Q8>(p, n_sm, st);
+}
+
+// 16-bit rows of q: the cache's own type where the cache is 16-bit.
+bool q_type_fits(int dtype, int kvd) {
+    return (dtype == ICUA_DT_F16 && kvd != ICUA_KV_BF16) || (dtype == ICUA_DT_BF16 && kvd != ICUA_KV_F16);
+}
+
+template <typename T, bool Q8>
+cudaError_t launch_attn(const PagedAttnParams& p, int dev, cudaStream_t st) {
+    const int smem = pa_smem(Q8);
+    cudaError_t e = allow_smem<paged_attn_kernel<T, Q8>>(smem, dev);
+    if (e != cudaSuccess) return e;
+    const int ctas = std::min(PA_MAX_CTAS, 2 * sm_count(dev));
+    paged_attn_kernel<T, Q8><<<ctas, PA_THREADS, smem, st>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(PA_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<T, pa_block(Q8)>, p, ctas);
+}
+
+icua_status check_attn(const icua_kv_pages* pages, const icua_kv_seqs* seqs, int32_t n_q, PagesView* P, SeqsView* S) {
+    const icua_status st = check_cache(pages, seqs, P, S);
+    if (st != ICUA_OK) return st;
+    if (n_q < pages->n_kv || n_q > 256 || n_q % pages->n_kv) return bad("n_q %d is not a multiple of n_kv %d up to 256", n_q, pages->n_kv);
+    // the kernels count blocks of keys over all items in 32 bits
+    const int64_t rows = (int64_t)seqs->total_q * (n_q / pages->n_kv);
+    const double blocks = ((double)rows / PA_ROWS + seqs->n_seqs) * pages->n_kv * ((double)seqs->max_pages * pages->page_size / 64 + 1);
+    if (rows > INT32_MAX || blocks > 4e9) return bad("the batch is too large: split it");
+    return ICUA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+icua_status icua_kv_write(const icua_kv_pages* pages, const icua_kv_seqs* seqs, const icua_kv_rows* rows, int32_t* err_dev,
+                          void* stream) {
+    KvWriteParams p{};
+    icua_status st = check_cache(pages, seqs, &p.pages, &p.seqs);
+    if (st != ICUA_OK) return st;
+    if (!rows || !rows->qkv || !aligned(rows->qkv, 16)) return bad("qkv is null or not 16-byte aligned");
+    if (rows->qkv_dtype < ICUA_DT_F32 || rows->qkv_dtype > ICUA_DT_F16) return bad("unknown qkv type %d", rows->qkv_dtype);
+    if (rows->n_q < 0 || rows->n_q > 256) return bad("n_q %d is not in 0..256", rows->n_q);
+    if (!q_type_fits(rows->q_dtype, pages->dtype)) return bad("q type %d does not go with cache type %d", rows->q_dtype, pages->dtype);
+    const int64_t width = (int64_t)(rows->n_q + 2 * pages->n_kv) * HD;
+    p.qkv_stride = rows->qkv_stride ? rows->qkv_stride : width;
+    p.q_stride = rows->q_stride ? rows->q_stride : (int64_t)rows->n_q * HD;
+    if (p.qkv_stride < width || p.qkv_stride % 8 || p.q_stride < (int64_t)rows->n_q * HD || p.q_stride % 8)
+        return bad("token strides are multiples of 8, at least a row (or 0)");
+    if (!aligned(rows->q_out, 16) || !aligned(rows->q_norm, 16) || !aligned(rows->k_norm, 16) || !aligned(rows->rope, 16) ||
+        !aligned(rows->rope_rows, 4) || !aligned(err_dev, 4))
+        return bad("a row array is not aligned");
+    if (rows->rope && rows->rope_len < 0) return bad("rope_len is negative");
+    if (!(rows->eps >= 0.f)) return bad("eps is negative or NaN");
+    if ((int64_t)seqs->total_q * (rows->n_q + 2 * pages->n_kv) > ((int64_t)16 << 31) - 16) return bad("the batch is too large: split it");
+    if (seqs->n_seqs == 0 || seqs->total_q == 0) return ICUA_OK;
+    int dev = 0;
+    if ((st = current(pages, rows->qkv, &dev)) != ICUA_OK) return st;
+    p.qkv = rows->qkv;
+    p.q_norm = rows->q_norm;
+    p.k_norm = rows->k_norm;
+    p.rope = reinterpret_cast<const float2*>(rows->rope);
+    p.rope_rows = rows->rope_rows;
+    p.rope_len = rows->rope_len;
+    p.n_q = rows->n_q;
+    p.eps = rows->eps;
+    p.q_out = rows->q_out;
+    p.err = err_dev;
+    cudaStream_t s = (cudaStream_t)stream;
+    const int n_sm = sm_count(dev);
+    const cudaError_t e = rows->qkv_dtype == ICUA_DT_F32    ? launch_write_in<float>(p, pages->dtype, rows->q_dtype, n_sm, s)
+                          : rows->qkv_dtype == ICUA_DT_BF16 ? launch_write_in<__nv_bfloat16>(p, pages->dtype, rows->q_dtype, n_sm, s)
+                                                            : launch_write_in<__half>(p, pages->dtype, rows->q_dtype, n_sm, s);
+    return e == cudaSuccess ? ICUA_OK : cuda_fail("icua_kv_write", e);
+}
+
+icua_status icua_kv_read(const icua_kv_pages* pages, const icua_kv_seqs* seqs, void* k_out, void* v_out, int32_t dtype,
+                         int32_t* err_dev, void* stream) {
+    KvReadParams p{};
+    icua_status st = check_cache(pages, seqs, &p.pages, &p.seqs);
+    if (st != ICUA_OK) return st;
+    if (dtype < ICUA_DT_F32 || dtype > ICUA_DT_F16) return bad("unknown row type %d", dtype);
+    if ((!k_out && !v_out) || !aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(err_dev, 4))
+        return bad("both outputs are null, or one is not 16-byte aligned");
+    if ((int64_t)seqs->total_q * 2 * pages->n_kv > ((int64_t)16 << 31) - 16) return bad("the batch is too large: split it");
+    if (seqs->n_seqs == 0 || seqs->total_q == 0) return ICUA_OK;
+    int dev = 0;
+    if ((st = current(pages, k_out ? k_out : v_out, &dev)) != ICUA_OK) return st;
+    p.k_out = k_out;
+    p.v_out = v_out;
+    p.err = err_dev;
+    cudaStream_t s = (cudaStream_t)stream;
+    const int n_sm = sm_count(dev);
+    const cudaError_t e = dtype == ICUA_DT_F32    ? launch_read<float>(p, pages->dtype, n_sm, s)
+                          : dtype == ICUA_DT_BF16 ? launch_read<__nv_bfloat16>(p, pages->dtype, n_sm, s)
+                                                  : launch_read<__half>(p, pages->dtype, n_sm, s);
+    return e == cudaSuccess ? ICUA_OK : cuda_fail("icua_kv_read", e);
+}
+
+uint64_t icua_attn_paged_scratch_bytes(const icua_kv_pages* pages, const icua_kv_seqs* seqs, int32_t n_q) {
+    PagesView P;
+    SeqsView S;
+    if (check_attn(pages, seqs, n_q, &P, &S) != ICUA_OK) return 0;
+    return (uint64_t)PA_MAX_CTAS * 2 * PA_PART * sizeof(float);
+}
+
+icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs, const icua_attn_paged_args* a, int32_t* err_dev,
+                            void* stream) {
+    PagedAttnParams p{};
+    if (!a) return bad("null argument");
+    icua_status st = check_attn(pages, seqs, a->n_q, &p.pages, &p.seqs);
+    if (st != ICUA_OK) return st;
+    if (!a->q || !a->out || !aligned(a->q, 16) || !aligned(a->out, 16) || !aligned(err_dev, 4))
+        return bad("q or out is null or not 16-byte aligned");
+    if (!q_type_fits(a->dtype, pages->dtype)) return bad("row type %d does not go with cache type %d", a->dtype, pages->dtype);
+    p.q_stride = a->q_stride ? a->q_stride : (int64_t)a->n_q * HD;
+    p.out_stride = a->out_stride ? a->out_stride : (int64_t)a->n_q * HD;
+    if (p.q_stride < (int64_t)a->n_q * HD || p.q_stride % 8 || p.out_stride < (int64_t)a->n_q * HD || p.out_stride % 8)
+        return bad("token strides are multiples of 8, at least a row (or 0)");
+    if (!(a->scale >= 0.f) || a->scale > 3e38f) return bad("scale is negative or not finite");
+    if (!a->scratch || !aligned(a->scratch, 16) || a->scratch_bytes < icua_attn_paged_scratch_bytes(pages, seqs, a->n_q))
+        return bad("scratch is null, not 16-byte aligned or smaller than icua_attn_paged_scratch_bytes");
+    if (seqs->n_seqs == 0 || seqs->total_q == 0) return ICUA_OK;
+    int dev = 0;
+    if ((st = current(pages, a->q, &dev)) != ICUA_OK) return st;
+    p.q = a->q;
+    p.out = a->out;
+    p.n_q = a->n_q;
+    p.group = a->n_q / pages->n_kv;
+    p.scale_log2 = (a->scale > 0.f ? a->scale : 0.08838834764831845f) * 1.4426950408889634f;
+    p.max_rows = INT32_MAX;
+    p.part = (float*)a->scratch;
+    p.err = err_dev;
+    cudaStream_t s = (cudaStream_t)stream;
+    const bool f16 = a->dtype == ICUA_DT_F16;
+    const cudaError_t e = pages->dtype == ICUA_KV_Q8 ? (f16 ? launch_attn<__half, true>(p, dev, s) : launch_attn<__nv_bfloat16, true>(p, dev, s))
+                          : f16                      ? launch_attn<__half, false>(p, dev, s)
+                                                     : launch_attn<__nv_bfloat16, false>(p, dev, s);
+    return e == cudaSuccess ? ICUA_OK : cuda_fail("icua_attn_paged", e);
+}
+
+}  // extern "C"

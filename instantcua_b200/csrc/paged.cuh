@@ -1,0 +1,347 @@
+// Paged K/V cache: the kernels that write new tokens into it (per-head norms and rotation in the
+// same pass, quantised as they are written) and read them back, and the device view of a cache and
+// its batch that these and the attention kernels share.
+//
+// A page holds page_size positions of every kv head; row (page, head, position in page) is row
+// page * page_rows + head * head_rows + position of the K and of the V pool.  16-bit rows are 256 B
+// in the engine's cache order (kv_swz); q8 rows are 128 int8 codes in plain order with one fp32
+// scale per row in a second array under the same row number.
+#pragma once
+#include "common.cuh"
+#include "warp_mma.cuh"
+
+namespace icua {
+
+enum KvDtype : int { KV_F16 = 0, KV_BF16 = 1, KV_Q8 = 2 };   // ICUA_KV_*
+enum RowDtype : int { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };  // ICUA_DT_*
+
+// Flags of the paged kernels in the caller's error word (beside the ERR_WAIT_* ones).
+enum : int { ERR_PAGE = 16, ERR_SEQ = 32 };
+
+struct PagesView {
+    uint8_t *k, *v;
+    float *ks, *vs;
+    long long page_rows, head_rows;
+    int n_kv, ps_shift, n_pages;
+};
+
+struct SeqsView {
+    const int *cu_q, *kv_len, *table;
+    int n_seqs, total_q, max_pages;
+};
+
+struct SeqInfo {
+    int q0, n, kv;  // first row, new tokens, positions in all
+};
+
+// A sequence's entry, checked: anything that would lead out of the row arrays or the page table
+// makes the sequence an empty one and raises ERR_SEQ.
+__device__ __forceinline__ SeqInfo load_seq(const SeqsView& S, int ps_shift, int s, int* err) {
+    const int q0 = S.cu_q[s], q1 = S.cu_q[s + 1], kv = S.kv_len[s];
+    if (q0 < 0 || q1 < q0 || q1 > S.total_q || kv < 0 || kv > ((long long)S.max_pages << ps_shift)) {
+        if (err) atomicOr(err, ERR_SEQ);
+        return SeqInfo{0, 0, 0};
+    }
+    return SeqInfo{q0, q1 - q0, kv};
+}
+
+// First pool row of position pos (any position of one page) of head h in sequence s, or -1 for a
+// table entry that names no page.
+__device__ __forceinline__ long long page_row(const PagesView& P, const SeqsView& S, int s, int h, int pos, int* err) {
+    const int page = S.table[(long long)s * S.max_pages + (pos >> P.ps_shift)];
+    if ((unsigned)page >= (unsigned)P.n_pages) {
+        if (err) atomicOr(err, ERR_PAGE);
+        return -1;
+    }
+    return page * P.page_rows + h * P.head_rows + (pos & ((1 << P.ps_shift) - 1));
+}
+
+// Sequence of row t: the number of sequences that end at or before t (cu_q ascends), counted by
+// the whole warp, 32 entries a round.
+__device__ __forceinline__ int find_seq(const SeqsView& S, int t, int lane) {
+    int c = 0;
+    for (int i = 0; i < S.n_seqs; i += 32) {
+        const bool le = i + lane < S.n_seqs && S.cu_q[i + lane + 1] <= t;
+        const unsigned b = __ballot_sync(0xffffffffu, le);
+        c += __popc(b);
+        if (b != 0xffffffffu) break;
+    }
+    return c;
+}
+
+struct KvWriteParams {
+    PagesView pages;
+    SeqsView seqs;
+    const void* qkv;
+    long long qkv_stride;  // elements between the rows of two tokens
+    const float *q_norm, *k_norm;
+    const float2* rope;
+    const int* rope_rows;
+    int rope_len, n_q;
+    float eps;
+    void* q_out;
+    long long q_stride;
+    int n_groups;  // half-warps per token, each for VPT consecutive head vectors
+    int* err;
+};
+
+// Eight consecutive elements (one 16-byte chunk of a 16-bit row) as floats.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]);
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+template <>
+__device__ __forceinline__ void load8<__half>(const __half* p, float (&x)[8]) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+template <>
+__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[8]) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_f(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack_f<__half>(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack_f<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack_f<T>(x[0], x[1]), pack_f<T>(x[2], x[3]), pack_f<T>(x[4], x[5]), pack_f<T>(x[6], x[7]));
+}
+template <>
+__device__ __forceinline__ void store8<float>(float* p, const float (&x)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+
+// One half-warp per head vector, 16 lanes x 8 elements: y = x rsqrt(mean x^2 + eps) w, then the
+// rotation of the pairs (j, j + 64) (the partner's eight are eight lanes away), both in fp32; q rows
+// are rounded to the output type, k and v rows to the cache type or to int8 codes: scale = max|x| /
+// 127 in fp32 and code = x / scale to the nearest even, so a code is off by at most half a step.  A
+// row that holds a NaN or an infinity gets the scale NaN and reads back as NaN throughout.  A row
+// of zeros gets the scale 1.
+// Bound: HBM for many tokens (each row read once and written once), latency for few, so a half-warp
+// takes VPT = 4 consecutive vectors of a token (its loads issued together, the sequence lookup and
+// the rotation row shared) where that still fills the GPU and one otherwise.
+template <typename TI, typename TQ, int KVD, int VPT>
+__global__ void __launch_bounds__(256) kv_write_kernel(const KvWriteParams p) {
+    using TC = typename std::conditional<KVD == KV_BF16, __nv_bfloat16, __half>::type;
+    const int lane = threadIdx.x & 31, l = lane & 15;
+    const long long unit = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;
+    const int t = (int)(unit / p.n_groups), v0 = (int)(unit % p.n_groups) * VPT;
+    // both halves' tokens, looked up by the whole warp
+    const int ta = __shfl_sync(0xffffffffu, t, 0), tb = __shfl_sync(0xffffffffu, t, 16);
+    const int sa = find_seq(p.seqs, ta, lane);
+    const int sb = tb == ta ? sa : find_seq(p.seqs, tb, lane);
+    const int s = lane < 16 ? sa : sb;
+    const int n_kv = p.pages.n_kv, n_vec = p.n_q + 2 * n_kv;
+    bool live = t < p.seqs.total_q && s < p.seqs.n_seqs;
+    int pos = 0;
+    if (live) {
+        const SeqInfo q = load_seq(p.seqs, p.pages.ps_shift, s, l == 0 ? p.err : nullptr);
+        pos = q.kv - q.n + (t - q.q0);
+        live = t >= q.q0 && t < q.q0 + q.n;
+        if (live && pos < 0) {  // more new tokens than positions: this one has no place
+            live = false;
+            if (p.err && l == 0) atomicOr(p.err, ERR_SEQ);
+        }
+    }
+    float cs[8], sn[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        cs[e] = 1.f;
+        sn[e] = 0.f;
+    }
+    if (live && p.rope != nullptr) {
+        const int r = p.rope_rows != nullptr ? p.rope_rows[t] : pos;
+        if ((unsigned)r >= (unsigned)p.rope_len) {
+            live = false;
+            if (p.err && l == 0) atomicOr(p.err, ERR_SEQ);
+        } else {
+            const float4* c4 = reinterpret_cast<const float4*>(p.rope + (long long)r * 64 + 8 * (l & 7));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float4 c = c4[e];
+                cs[2 * e] = c.x; sn[2 * e] = c.y;
+                cs[2 * e + 1] = c.z; sn[2 * e + 1] = c.w;
+            }
+        }
+    }
+    if (l < 8) {  // the first half of a pair turns by -sin
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sn[e] = -sn[e];
+    }
+    float x[VPT][8];
+    const TI* row = reinterpret_cast<const TI*>(p.qkv) + (long long)t * p.qkv_stride + 8 * l;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        if (live && v0 + i < n_vec) {
+            load8<TI>(row + (long long)(v0 + i) * HD, x[i]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+        }
+    }
+    long long crow = -1;  // pool row of kv head 0
+    if (live && v0 + VPT > p.n_q) crow = page_row(p.pages, p.seqs, s, 0, pos, l == 0 ? p.err : nullptr);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int vi = v0 + i;
+        const bool is_v = vi >= p.n_q + n_kv, is_q = vi < p.n_q;
+        const float* nw = is_v ? nullptr : is_q ? p.q_norm : p.k_norm;
+        if (nw != nullptr) {
+            float w[8];
+            load8<float>(nw + 8 * l, w);
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = fmaf(x[i][e], x[i][e], ss);
+            const unsigned half_mask = lane < 16 ? 0x0000ffffu : 0xffff0000u;
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(half_mask, ss, o);
+            const float r = 1.0f / sqrtf(ss / (float)HD + p.eps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[i][e] = x[i][e] * r * w[e];
+        }
+        __syncwarp();
+        if (p.rope != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float other = __shfl_xor_sync(0xffffffffu, x[i][e], 8);
+                if (!is_v) x[i][e] = x[i][e] * cs[e] + other * sn[e];
+            }
+        }
+        float amax = 0.f;
+        bool bad = false;
+        if (KVD == KV_Q8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                amax = fmaxf(amax, fabsf(x[i][e]));
+                bad |= !(fabsf(x[i][e]) <= 3.402823466e38f);
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            const unsigned b = __ballot_sync(0xffffffffu, bad);
+            bad = (lane < 16 ? b & 0xffffu : b >> 16) != 0;
+        }
+        if (!live || vi >= n_vec) continue;
+        if (is_q) {
+            if (p.q_out != nullptr)
+                store8<TQ>(reinterpret_cast<TQ*>(p.q_out) + (long long)t * p.q_stride + vi * HD + 8 * l, x[i]);
+            continue;
+        }
+        if (crow < 0) continue;
+        const int h = is_v ? vi - p.n_q - n_kv : vi - p.n_q;
+        const long long r = crow + h * p.pages.head_rows;
+        uint8_t* pool = is_v ? p.pages.v : p.pages.k;
+        if (KVD == KV_Q8) {
+            float sc = amax / 127.0f;
+            if (sc == 0.f) sc = 1.f;
+            uint32_t c[2] = {0u, 0u};
+            if (!bad) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int q = max(-127, min(127, __float2int_rn(x[i][e] / sc)));
+                    c[e >> 2] |= (uint32_t)(q & 0xff) << (8 * (e & 3));
+                }
+            }
+            *reinterpret_cast<uint2*>(pool + r * HD + 8 * l) = make_uint2(c[0], c[1]);
+            if (l == 0) (is_v ? p.pages.vs : p.pages.ks)[r] = bad ? __int_as_float(0x7fc00000) : sc;
+        } else {
+            store8<TC>(reinterpret_cast<TC*>(pool) + r * HD + 8 * (l ^ (pos & 7)), x[i]);
+        }
+    }
+}
+
+struct KvReadParams {
+    PagesView pages;
+    SeqsView seqs;
+    void *k_out, *v_out;
+    int n_groups;  // half-warps per token, each for VPT of its 2 n_kv rows
+    int* err;
+};
+
+// value = code * scale (q8) or the stored 16-bit value, one rounding to the output type.  A row of a
+// position that the sequence does not have, or of a table entry that names no page, reads as zeros.
+// Bound: HBM; a half-warp has VPT rows of one token in flight.
+template <typename TO, int KVD, int VPT>
+__global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p) {
+    using TC = typename std::conditional<KVD == KV_BF16, __nv_bfloat16, __half>::type;
+    const int lane = threadIdx.x & 31, l = lane & 15;
+    const long long unit = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;
+    const int t = (int)(unit / p.n_groups), v0 = (int)(unit % p.n_groups) * VPT;
+    const int ta = __shfl_sync(0xffffffffu, t, 0), tb = __shfl_sync(0xffffffffu, t, 16);
+    const int sa = find_seq(p.seqs, ta, lane);
+    const int sb = tb == ta ? sa : find_seq(p.seqs, tb, lane);
+    const int s = lane < 16 ? sa : sb;
+    if (t >= p.seqs.total_q || s >= p.seqs.n_seqs) return;
+    const int n_kv = p.pages.n_kv;
+    const SeqInfo q = load_seq(p.seqs, p.pages.ps_shift, s, l == 0 ? p.err : nullptr);
+    if (t < q.q0 || t >= q.q0 + q.n) return;
+    const int pos = q.kv - q.n + (t - q.q0);
+    long long crow = -1;
+    if (pos >= 0) crow = page_row(p.pages, p.seqs, s, 0, pos, l == 0 ? p.err : nullptr);
+    else if (p.err && l == 0) atomicOr(p.err, ERR_SEQ);
+    uint4 raw[VPT];
+    float sc[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int vi = v0 + i, h = vi < n_kv ? vi : vi - n_kv;
+        raw[i] = make_uint4(0, 0, 0, 0);
+        sc[i] = 0.f;
+        if (vi < 2 * n_kv && crow >= 0) {
+            const long long r = crow + h * p.pages.head_rows;
+            const uint8_t* pool = vi < n_kv ? p.pages.k : p.pages.v;
+            if (KVD == KV_Q8) {
+                const uint2 c = *reinterpret_cast<const uint2*>(pool + r * HD + 8 * l);
+                raw[i].x = c.x;
+                raw[i].y = c.y;
+                sc[i] = (vi < n_kv ? p.pages.ks : p.pages.vs)[r];
+            } else {
+                raw[i] = *reinterpret_cast<const uint4*>(pool + r * 2 * HD + 16 * (l ^ (pos & 7)));
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int vi = v0 + i, h = vi < n_kv ? vi : vi - n_kv;
+        if (vi >= 2 * n_kv) break;
+        TO* o = reinterpret_cast<TO*>(vi < n_kv ? p.k_out : p.v_out);
+        if (o == nullptr) continue;
+        float x[8];
+        if (KVD == KV_Q8) {
+            const uint32_t c[2] = {raw[i].x, raw[i].y};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (float)(int8_t)(c[e >> 2] >> (8 * (e & 3))) * sc[i];
+        } else {
+            load8<TC>(reinterpret_cast<const TC*>(&raw[i]), x);
+        }
+        store8<TO>(o + ((long long)t * n_kv + h) * HD + 8 * l, x);
+    }
+}
+
+}  // namespace icua
