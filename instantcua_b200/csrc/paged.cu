@@ -1,5 +1,6 @@
 // Entry points of the paged K/V cache (include/icua.h): argument checks, choice of the kernel
-// variant and launch.  Kernels: paged.cuh (write, read back), paged_attn.cuh (attention).
+// variant and launch.  Kernels: paged.cuh (write, read back), paged_attn.cuh and paged_attn_tc.cuh
+// (attention of few and of many rows).
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
@@ -8,6 +9,7 @@
 #include "../../include/icua.h"
 #include "paged.cuh"
 #include "paged_attn.cuh"
+#include "paged_attn_tc.cuh"
 
 namespace icua_host {
 icua_status set_global_error(icua_status s, const char* msg);
@@ -171,6 +173,42 @@ cudaError_t launch_attn(const PagedAttnParams& p, int dev, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<T, pa_block(Q8)>, p, ctas);
 }
 
+// Tiles of the tensor-core kernel: a bound from what the host knows, and the shares of the keys that fill
+// the SMs when the tiles alone do not (two blocks of keys per share at least).
+constexpr int PC_MAX_SHARES = 160;
+struct TcGrid {
+    int tiles, n_split;
+};
+TcGrid tc_grid(const icua_kv_seqs* s, int n_kv, int group, int min_rows, int n_sm) {
+    const int64_t rows = (int64_t)s->total_q * group;
+    TcGrid g;
+    g.tiles = (int)(rows / PC_ROWS + std::min<int64_t>(s->n_seqs, rows / (min_rows + 1)));
+    const int base = g.tiles * n_kv;
+    g.n_split = std::max(1, std::min(std::min(n_sm, PC_MAX_SHARES) / std::max(base, 1), (s->max_kv + 2 * PC_BK - 1) / (2 * PC_BK)));
+    return g;
+}
+
+template <typename T, bool Q8>
+cudaError_t launch_attn_tc(const PagedTcParams& p, int tiles, int dev, cudaStream_t st) {
+    cudaError_t e = allow_smem<paged_attn_tc_kernel<T, Q8>>(PcSmem::alloc, dev);
+    if (e != cudaSuccess) return e;
+    paged_attn_tc_kernel<T, Q8><<<tiles * p.pages.n_kv * p.n_split, PC_THREADS, PcSmem::alloc, st>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess || p.n_split == 1) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(tiles * p.pages.n_kv * 32);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, paged_attn_tc_join_kernel<T>, p);
+}
+
+constexpr size_t PA_SCRATCH = (size_t)PA_MAX_CTAS * 2 * PA_PART * sizeof(float);
+constexpr size_t PC_SCRATCH = (size_t)PC_MAX_SHARES * PC_PART * sizeof(float);
+
 icua_status check_attn(const icua_kv_pages* pages, const icua_kv_seqs* seqs, int32_t n_q, PagesView* P, SeqsView* S) {
     const icua_status st = check_cache(pages, seqs, P, S);
     if (st != ICUA_OK) return st;
@@ -254,7 +292,7 @@ uint64_t icua_attn_paged_scratch_bytes(const icua_kv_pages* pages, const icua_kv
     PagesView P;
     SeqsView S;
     if (check_attn(pages, seqs, n_q, &P, &S) != ICUA_OK) return 0;
-    return (uint64_t)PA_MAX_CTAS * 2 * PA_PART * sizeof(float);
+    return PA_SCRATCH + ((int64_t)seqs->max_q * (n_q / pages->n_kv) > PA_ROWS ? PC_SCRATCH : 0);
 }
 
 icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs, const icua_attn_paged_args* a, int32_t* err_dev,
@@ -281,14 +319,43 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
     p.n_q = a->n_q;
     p.group = a->n_q / pages->n_kv;
     p.scale_log2 = (a->scale > 0.f ? a->scale : 0.08838834764831845f) * 1.4426950408889634f;
-    p.max_rows = INT32_MAX;
+    p.max_rows = PA_ROWS;
     p.part = (float*)a->scratch;
     p.err = err_dev;
     cudaStream_t s = (cudaStream_t)stream;
-    const bool f16 = a->dtype == ICUA_DT_F16;
-    const cudaError_t e = pages->dtype == ICUA_KV_Q8 ? (f16 ? launch_attn<__half, true>(p, dev, s) : launch_attn<__nv_bfloat16, true>(p, dev, s))
-                          : f16                      ? launch_attn<__half, false>(p, dev, s)
-                                                     : launch_attn<__nv_bfloat16, false>(p, dev, s);
+    const bool f16 = a->dtype == ICUA_DT_F16, q8 = pages->dtype == ICUA_KV_Q8;
+    cudaError_t e = cudaSuccess;
+    // Sequences of up to 16 query rows per kv head go through the warp-MMA kernel, which reads the cache
+    // at HBM speed whatever the rows; more rows through the tensor-core kernel.
+    const bool tc = (int64_t)seqs->max_q * p.group > PA_ROWS;
+    // A batch whose sequences all seem to bring max_q tokens goes there whole, one launch less (a shorter
+    // sequence that it holds all the same is then a tile like any other).
+    const bool all_tc = tc && (int64_t)seqs->n_seqs * seqs->max_q == seqs->total_q;
+    if (tc) {
+        PagedTcParams c{};
+        c.pages = p.pages;
+        c.seqs = p.seqs;
+        c.q = p.q;
+        c.out = p.out;
+        c.q_stride = p.q_stride;
+        c.out_stride = p.out_stride;
+        c.group = p.group;
+        c.scale_log2 = p.scale_log2;
+        c.min_rows = all_tc ? 0 : PA_ROWS;
+        c.part = (float*)((uint8_t*)a->scratch + PA_SCRATCH);
+        c.err = err_dev;
+        const TcGrid g = tc_grid(seqs, pages->n_kv, p.group, c.min_rows, sm_count(dev));
+        c.n_split = g.n_split;
+        if (g.tiles > 0)
+            e = q8 ? (f16 ? launch_attn_tc<__half, true>(c, g.tiles, dev, s) : launch_attn_tc<__nv_bfloat16, true>(c, g.tiles, dev, s))
+                : f16 ? launch_attn_tc<__half, false>(c, g.tiles, dev, s)
+                      : launch_attn_tc<__nv_bfloat16, false>(c, g.tiles, dev, s);
+    }
+    p.alone = !tc;
+    if (e == cudaSuccess && !all_tc)
+        e = q8 ? (f16 ? launch_attn<__half, true>(p, dev, s) : launch_attn<__nv_bfloat16, true>(p, dev, s))
+            : f16 ? launch_attn<__half, false>(p, dev, s)
+                  : launch_attn<__nv_bfloat16, false>(p, dev, s);
     return e == cudaSuccess ? ICUA_OK : cuda_fail("icua_attn_paged", e);
 }
 

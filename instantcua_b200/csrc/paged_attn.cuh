@@ -44,7 +44,8 @@ struct PagedAttnParams {
     long long q_stride, out_stride;
     int n_q, group;
     float scale_log2;  // softmax scale x log2(e)
-    int max_rows;      // sequences with more rows (n G) than this belong to another kernel
+    int max_rows;      // sequences with more rows (n G) than this belong to another kernel,
+    int alone;         //   or, when there is none in this call, break the caller's max_q (ERR_SEQ)
     float* part;       // [gridDim.x][2][PA_PART]: 0 = an item begun by an earlier CTA, 1 = an item begun here
     int* err;
 };
@@ -92,7 +93,7 @@ struct PaWork {
     int n, kv, q0, tiles, nb, items;
 };
 __device__ __forceinline__ PaWork pa_work(const SeqsView& S, int ps_shift, int n_kv, int group, int max_rows, int block, int s,
-                                          int* err) {
+                                          int* err, bool alone = false) {
     const SeqInfo q = load_seq(S, ps_shift, s, err);
     PaWork w{q.n, q.kv, q.q0, 0, 0, 0};
     const long long rows = (long long)q.n * group;
@@ -100,6 +101,8 @@ __device__ __forceinline__ PaWork pa_work(const SeqsView& S, int ps_shift, int n
         w.tiles = (int)((rows + PA_ROWS - 1) / PA_ROWS);
         w.items = w.tiles * n_kv;
         w.nb = max(1, (q.kv + block - 1) / block);  // an item without keys still writes its (zero) rows
+    } else if (rows > 0 && alone && err) {
+        atomicOr(err, ERR_SEQ);
     }
     return w;
 }
@@ -107,14 +110,14 @@ __device__ __forceinline__ PaWork pa_work(const SeqsView& S, int ps_shift, int n
 // pre[s] = blocks before sequence s, pre[n_seqs] = all of them.  `warp_tot` holds one word per warp.
 template <int THREADS>
 __device__ __forceinline__ uint32_t pa_prefix(const SeqsView& S, int ps_shift, int n_kv, int group, int max_rows, int block,
-                                              uint32_t* pre, uint32_t* warp_tot, int* err) {
+                                              uint32_t* pre, uint32_t* warp_tot, int* err, bool alone = false) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint32_t base = 0;
     for (int s0 = 0; s0 < S.n_seqs; s0 += THREADS) {
         const int s = s0 + tid;
         uint32_t w = 0;
         if (s < S.n_seqs) {
-            const PaWork k = pa_work(S, ps_shift, n_kv, group, max_rows, block, s, err);
+            const PaWork k = pa_work(S, ps_shift, n_kv, group, max_rows, block, s, err, alone);
             w = (uint32_t)k.items * (uint32_t)k.nb;
         }
         uint32_t x = w;
@@ -150,9 +153,17 @@ __device__ __forceinline__ int pa_find(const uint32_t* pre, int n, uint32_t x) {
     return lo;
 }
 
-__host__ __device__ __forceinline__ uint32_t pa_begin(uint32_t total, uint32_t c, uint32_t ctas) {
-    return (uint32_t)((unsigned long long)total * c / ctas);
-}
+// The line dealt to the CTAs: the first r take q + 1 blocks, the others q (none past the end of a line
+// that is shorter than the grid).
+struct PaDeal {
+    uint32_t q, r;
+    __device__ __forceinline__ PaDeal(uint32_t total, uint32_t ctas) : q(total / ctas), r(total % ctas) {}
+    __device__ __forceinline__ uint32_t begin(uint32_t c) const { return c * q + min(c, r); }
+    __device__ __forceinline__ uint32_t cta_of(uint32_t x) const {
+        const uint32_t lead = r * (q + 1);
+        return x < lead ? x / (q + 1) : r + (x - lead) / max(q, 1u);
+    }
+};
 
 template <typename T, bool Q8>
 __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAttnParams p) {
@@ -165,8 +176,10 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int ps_shift = p.pages.ps_shift, n_kv = p.pages.n_kv, G = p.group;
     const uint32_t total =
-        pa_prefix<PA_THREADS>(p.seqs, ps_shift, n_kv, G, p.max_rows, BLOCK, pre, warp_tot, blockIdx.x == 0 ? p.err : nullptr);
-    const uint32_t x0 = pa_begin(total, blockIdx.x, gridDim.x), x1 = pa_begin(total, blockIdx.x + 1, gridDim.x);
+        pa_prefix<PA_THREADS>(p.seqs, ps_shift, n_kv, G, p.max_rows, BLOCK, pre, warp_tot, blockIdx.x == 0 ? p.err : nullptr,
+                               p.alone != 0);
+    const PaDeal deal(total, gridDim.x);
+    const uint32_t x0 = deal.begin(blockIdx.x), x1 = deal.begin(blockIdx.x + 1);
     pdl_launch_dependents();
     if (x0 >= x1) return;
 
@@ -526,14 +539,14 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const Paged
     __shared__ uint32_t warp_tot[PA_WARPS];
     const int tid = threadIdx.x, G = p.group;
     const uint32_t total = pa_prefix<PA_THREADS>(p.seqs, p.pages.ps_shift, p.pages.n_kv, G, p.max_rows, BLOCK, pre, warp_tot, nullptr);
-    const uint32_t c0 = blockIdx.x, x0 = pa_begin(total, c0, ctas), x1 = pa_begin(total, c0 + 1, ctas);
+    const PaDeal deal(total, ctas);
+    const uint32_t c0 = blockIdx.x, x0 = deal.begin(c0), x1 = deal.begin(c0 + 1);
     if (x0 >= x1) return;
     const int s = pa_find(pre, p.seqs.n_seqs, x1 - 1);
     const PaWork w = pa_work(p.seqs, p.pages.ps_shift, p.pages.n_kv, G, p.max_rows, BLOCK, s, nullptr);
     const uint32_t item = (x1 - 1 - pre[s]) / w.nb, i0 = pre[s] + item * w.nb, i1 = i0 + w.nb;
     if (i0 < x0 || i1 <= x1) return;
-    uint32_t c1 = c0 + 1;  // the CTA of the item's last block
-    while (pa_begin(total, c1 + 1, ctas) < i1) ++c1;
+    const uint32_t c1 = deal.cta_of(i1 - 1);
     const int h = item / w.tiles, tile = item % w.tiles, rows = min(PA_ROWS, w.n * G - tile * PA_ROWS);
     pdl_wait();
     // thread = four columns of every fourth row
@@ -543,7 +556,6 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const Paged
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
         for (uint32_t c = c0; c <= c1; ++c) {
-            if (c > c0 && pa_begin(total, c, ctas) == pa_begin(total, c + 1, ctas)) continue;  // a CTA without blocks
             const float* pt = p.part + (size_t)(2 * c + (c == c0 ? 1 : 0)) * PA_PART;
             const float pm = pt[PA_ROWS * HD + r], pl = pt[PA_ROWS * HD + PA_ROWS + r];
             const float4 v = *reinterpret_cast<const float4*>(pt + r * HD + col);

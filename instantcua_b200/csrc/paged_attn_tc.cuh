@@ -1,0 +1,534 @@
+// Attention of chunks and prompts over a paged K/V cache on the 5th-generation tensor cores.
+//
+// The n G query rows of a (sequence, kv head) (row r = token r / G, head r % G) are cut into tiles of 2
+// x 128; one CTA takes a tile over all its keys, or over a share of them (n_split) when there are fewer
+// tiles than SMs.  Per block of 128 keys and half t:
+//   S_t = Q_t K^T     (M = 128, N = 128, K = 128; both operands K-major in shared memory)
+//   P_t = 2^(S_t scale log2(e) - m)   in the 16-bit type of q, written over S_t in tensor memory
+//   O_t += P_t V      (A = P_t from tensor memory, B = V as it lies in the cache: MN-major)
+// warps 0-3 / 4-7  softmax of half 0 / 1, one thread per row (tensor-memory lane)
+// warp 8           tensor memory, and the one thread that issues every product
+// warps 9-12       bring the q rows and the K / V blocks: 16-bit rows by cp.async into the 128-byte
+//                  swizzle (which is the cache's own row order), q8 rows through registers, converted
+//                  exactly; rows past the sequence's end and of pages that do not exist are zeros
+// While one half's softmax runs, the tensor core works for the other half.  The running maximum is
+// only moved (and O_t rescaled in tensor memory) when a score exceeds it by more than 2^8: P then stays
+// below 256, which the 16-bit types hold as precisely as 1, and the rescale is rare.
+// q8 caches: the scales enter as in paged_attn.cuh, as three fp32 factors per key.
+// Bound: the exponentials (16 per clock and SM: 1,024 clocks per 128 x 128 scores, as many as its two
+// products take) and the tensor core.
+// Every wait is bounded: one that gives up raises ERR_WAIT_PREFILL and the CTA still drains its copies
+// and products and frees its tensor memory.
+#pragma once
+#include "paged_attn.cuh"
+
+namespace icua {
+
+constexpr int PC_BK = 128;
+constexpr int PC_ROWS = 256;
+constexpr int PC_THREADS = 13 * 32;
+constexpr int PC_TMEM_COLS = 512;  // S / P of the halves at 0, 128; O at 256, 384
+constexpr int PC_PART = PC_ROWS * HD + 2 * PC_ROWS;  // floats of a part: o[256][128], m[256], l[256]
+
+struct PcSmem {
+    static constexpr int q_off = 0;                       // 2 halves x [2][128 rows][128 B]
+    static constexpr int k_off = 65536;                   // 2 stages x [2][128 keys][128 B]
+    static constexpr int v_off = k_off + 2 * 32768;
+    static constexpr int c_off = v_off + 2 * 32768;       // q8: 4 x (mul, add, inv)[128]
+    static constexpr int bar_off = c_off + 4 * 3 * 512;
+    static constexpr int total = bar_off + 20 * 8;
+    static constexpr int alloc = total + 1024;
+};
+
+struct PagedTcParams {
+    PagesView pages;
+    SeqsView seqs;
+    const void* q;
+    void* out;
+    long long q_stride, out_stride;
+    int group;
+    float scale_log2;
+    int min_rows;  // sequences with at most so many rows belong to the other kernel
+    int n_split;
+    float* part;   // [gridDim.x][PC_PART] when n_split > 1
+    int* err;
+};
+
+// Shared-memory descriptor of an MN-major operand in the 128-byte swizzle: 64-element groups of the M / N
+// index `lbo` bytes apart, groups of eight K rows 1,024 bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t saddr, uint32_t lbo) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+template <typename T>
+__host__ __device__ constexpr uint32_t pc_idesc(bool b_mn) {
+    return umma_idesc_f16(128, 128) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+    uint32_t a[16], b[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        a[i] = __float_as_uint(v[i]);
+        b[i] = __float_as_uint(v[16 + i]);
+    }
+    tmem_st16(taddr, a);
+    tmem_st16(taddr + 16, b);
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Tile of the grid: which rows of which sequence, and the keys its share covers.
+struct PcTile {
+    int s, q0, n, kv, row0;  // row0: first of the tile's 256 query rows
+    int j0, j1, last;        // blocks of keys [j0, j1); the last key any row sees
+};
+
+// The y-th tile of the batch (later tiles of a sequence, which see more keys, come first), found by one
+// warp.  False past the last one.
+__device__ __forceinline__ bool pc_find(const SeqsView& S, int ps_shift, int G, int min_rows, int y, int lane, PcTile& t, int* err) {
+    int before = 0;
+    for (int s0 = 0; s0 < S.n_seqs; s0 += 32) {
+        SeqInfo q{0, 0, 0};
+        if (s0 + lane < S.n_seqs) q = load_seq(S, ps_shift, s0 + lane, err);
+        const int rows = q.n * G;
+        const int tiles = rows > min_rows ? (rows + PC_ROWS - 1) / PC_ROWS : 0;
+        int x = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int z = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += z;
+        }
+        const int all = __shfl_sync(0xffffffffu, x, 31);
+        if (y < before + all) {
+            const unsigned b = __ballot_sync(0xffffffffu, y < before + x);
+            const int src = __ffs(b) - 1;
+            t.s = s0 + src;
+            t.q0 = __shfl_sync(0xffffffffu, q.q0, src);
+            t.n = __shfl_sync(0xffffffffu, q.n, src);
+            t.kv = __shfl_sync(0xffffffffu, q.kv, src);
+            const int first = before + __shfl_sync(0xffffffffu, x - tiles, src);
+            const int cnt = __shfl_sync(0xffffffffu, tiles, src);
+            t.row0 = (cnt - 1 - (y - first)) * PC_ROWS;
+            return true;
+        }
+        before += all;
+    }
+    return false;
+}
+__device__ __forceinline__ void pc_share(PcTile& t, int G, int split, int n_split) {
+    t.last = t.kv - t.n + min(t.row0 + PC_ROWS - 1, t.n * G - 1) / G;
+    const int nb = t.last < 0 ? 0 : t.last / PC_BK + 1;
+    t.j0 = (int)((long long)nb * split / n_split);
+    t.j1 = (int)((long long)nb * (split + 1) / n_split);
+}
+
+// Grid: n_kv x n_split x (a bound of the) tiles, kv head fastest.
+template <typename T, bool Q8>
+__global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const PagedTcParams p) {
+    using S = PcSmem;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ PcTile tile_s;
+    __shared__ int live_s;
+    __shared__ uint32_t tmem_slot;
+    const uint32_t base_u = smem_u32(smem_raw);
+    uint8_t* smem = smem_raw + (((base_u + 1023u) & ~1023u) - base_u);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::bar_off);
+    uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7, *s_full = bars + 9,
+             *p_full = bars + 11, *o_full = bars + 13, *done = bars + 15, *c_full = bars + 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n_kv = p.pages.n_kv, G = p.group, ps_shift = p.pages.ps_shift;
+    const int h = blockIdx.x % n_kv, split = (blockIdx.x / n_kv) % p.n_split, y = blockIdx.x / (n_kv * p.n_split);
+
+    if (warp == 0) {
+        PcTile t{};
+        const bool live = pc_find(p.seqs, ps_shift, G, p.min_rows, y, lane, t, blockIdx.x == 0 ? p.err : nullptr);
+        if (live) pc_share(t, G, split, p.n_split);
+        if (lane == 0) {
+            tile_s = t;
+            live_s = live;
+        }
+    } else if (threadIdx.x == 32) {
+        mbar_init(q_full, 128);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], 128);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], 128);
+            mbar_init(&v_empty[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_full[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) mbar_init(&c_full[i], 128);
+        mbar_init(done, 1);
+        fence_mbar_init();
+    }
+    __syncthreads();
+    pdl_launch_dependents();
+    if (!live_s) return;
+    if (warp == 8) {
+        tmem_alloc(&tmem_slot, PC_TMEM_COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const PcTile t = tile_s;
+    const int rows = t.n * G, nblk = t.j1 - t.j0;
+    // blocks of the half: its last row sees no further
+    auto half_blocks = [&](int hf) {
+        const int r0 = t.row0 + 128 * hf;
+        if (r0 >= rows) return 0;
+        const int last = t.kv - t.n + min(r0 + 127, rows - 1) / G;
+        return last < 0 ? 0 : max(0, min(t.j1, last / PC_BK + 1) - t.j0);
+    };
+
+    if (warp >= 9) {
+        // ---- producers -----------------------------------------------------------------------------
+        const int w = warp - 9;
+        bool ok = true;
+        {
+            const T* qrow[2];
+            bool real[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {  // this warp's rows 64 w + lane, + 32
+                const int R = t.row0 + 64 * w + 32 * i + lane;
+                real[i] = R < rows;
+                const int tok = min(R, rows - 1) / G, hd = min(R, rows - 1) % G;
+                qrow[i] = reinterpret_cast<const T*>(p.q) + (t.q0 + tok) * p.q_stride + (h * G + hd) * HD;
+            }
+            const uint32_t qs = smem_u32(smem + S::q_off);
+            const int c = lane & 15;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const int src = 2 * k + (lane >> 4);
+                    const unsigned long long a = __shfl_sync(0xffffffffu, (unsigned long long)qrow[i], src);
+                    const bool rl = __shfl_sync(0xffffffffu, (int)real[i], src);
+                    const int R = 64 * w + 32 * i + src;  // row of the tile: half R / 128
+                    cp_async16(qs + (R >> 7) * 32768 + (c >> 3) * 16384 + (R & 127) * 128 + (((c & 7) ^ (R & 7)) << 4),
+                               reinterpret_cast<const uint8_t*>(a) + c * 16, rl);
+                }
+            cp_async_commit();
+            cp_async_wait<0>();
+            fence_proxy_async_smem();
+            mbar_arrive(q_full);
+        }
+        // pool row of key 32 w + lane of block j (all ones: none)
+        auto key_row = [&](int j) -> uint32_t {
+            const int pos = j * PC_BK + 32 * w + lane;
+            if (pos >= t.kv) return 0xffffffffu;
+            const long long r = page_row(p.pages, p.seqs, t.s, h, pos, p.err);
+            return r < 0 ? 0xffffffffu : (uint32_t)r;
+        };
+        if (!Q8) {
+            const int c = lane & 15;
+            auto issue = [&](uint8_t* dst, const uint8_t* pool, uint32_t row) {
+                const uint32_t d = smem_u32(dst) + (c >> 3) * 16384 + (c & 7) * 16 + (32 * w) * 128;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const int src = 2 * k + (lane >> 4);
+                    const uint32_t r = __shfl_sync(0xffffffffu, row, src);
+                    const bool rl = r != 0xffffffffu;
+                    cp_async16(d + src * 128, pool + (rl ? (size_t)r * 256 + c * 16 : 0), rl);
+                }
+                cp_async_commit();
+            };
+            uint32_t row = nblk > 0 ? key_row(t.j0) : 0;
+            for (int i = 0; i < nblk; ++i) {
+                const int st = i & 1;
+                const uint32_t next = i + 1 < nblk ? key_row(t.j0 + i + 1) : 0;
+                if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait_bounded(&k_empty[st], ((i >> 1) - 1) & 1))) { ok = false; break; }
+                issue(smem + S::k_off + st * 32768, p.pages.k, row);
+                if (i >= 1) {  // two copies stay in flight: K of the block before has landed
+                    cp_async_wait<2>();
+                    fence_proxy_async_smem();
+                    mbar_arrive(&k_full[(i - 1) & 1]);
+                }
+                if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait_bounded(&v_empty[st], ((i >> 1) - 1) & 1))) { ok = false; break; }
+                issue(smem + S::v_off + st * 32768, p.pages.v, row);
+                if (i >= 1) {
+                    cp_async_wait<2>();
+                    fence_proxy_async_smem();
+                    mbar_arrive(&v_full[(i - 1) & 1]);
+                }
+                row = next;
+            }
+            if (ok && nblk > 0) {
+                cp_async_wait<1>();
+                fence_proxy_async_smem();
+                mbar_arrive(&k_full[(nblk - 1) & 1]);
+                cp_async_wait<0>();
+                fence_proxy_async_smem();
+                mbar_arrive(&v_full[(nblk - 1) & 1]);
+            }
+            cp_async_wait<0>();
+        } else {
+            // eight 16-byte loads a lane: rows 4 i + lane / 8 of the warp's 32, chunk lane % 8
+            const int c = lane & 7;
+            uint4 rk[8], rv[8];
+            auto load = [&](uint4 (&raw)[8], const uint8_t* pool, uint32_t row) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t r = __shfl_sync(0xffffffffu, row, 4 * i + (lane >> 3));
+                    raw[i] = make_uint4(0, 0, 0, 0);
+                    if (r != 0xffffffffu) raw[i] = *reinterpret_cast<const uint4*>(pool + (size_t)r * HD + c * 16);
+                }
+            };
+            // 16 codes become two chunks of the 128-byte swizzle; the two halves of the row in turn, so that
+            // eight lanes store to eight different bank groups
+            auto store = [&](uint8_t* dst, const uint4 (&raw)[8]) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int R = 32 * w + 4 * i + (lane >> 3);
+                    const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                    uint32_t y[8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        y[2 * e] = codes_to_pair<T>(prmt(x[e], 0, 0x0100));
+                        y[2 * e + 1] = codes_to_pair<T>(prmt(x[e], 0, 0x0302));
+                    }
+                    uint8_t* d = dst + (c >> 2) * 16384 + R * 128;
+                    const int p0 = 2 * (c & 3);
+                    const bool odd = c >> 2;
+                    const uint4 lo = make_uint4(y[0], y[1], y[2], y[3]), hi = make_uint4(y[4], y[5], y[6], y[7]);
+                    *reinterpret_cast<uint4*>(d + (((p0 + odd) ^ (R & 7)) << 4)) = odd ? hi : lo;
+                    *reinterpret_cast<uint4*>(d + (((p0 + !odd) ^ (R & 7)) << 4)) = odd ? lo : hi;
+                }
+            };
+            uint32_t row = nblk > 0 ? key_row(t.j0) : 0xffffffffu;
+            load(rk, p.pages.k, row);
+            for (int i = 0; i < nblk; ++i) {
+                const int st = i & 1;
+                load(rv, p.pages.v, row);
+                const bool rl = row != 0xffffffffu;
+                const float ksc = rl ? p.pages.ks[row] : 0.f, vsc = rl ? p.pages.vs[row] : 1.f;
+                const uint32_t next = i + 1 < nblk ? key_row(t.j0 + i + 1) : 0xffffffffu;
+                if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait_bounded(&k_empty[st], ((i >> 1) - 1) & 1))) { ok = false; break; }
+                store(smem + S::k_off + st * 32768, rk);
+                {
+                    // (block i + 4 is stored after the scores of block i + 2, which come after both halves' softmax of i)
+                    float* f = reinterpret_cast<float*>(smem + S::c_off) + (i & 3) * 384 + 32 * w + lane;
+                    const float vs = vsc < 1e-37f ? 1e-37f : vsc;
+                    f[0] = ksc * p.scale_log2;
+                    f[128] = log2f(vs);
+                    f[256] = vs == vs ? 1.0f / vs : 0.f;
+                    mbar_arrive(&c_full[i & 3]);
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&k_full[st]);
+                load(rk, p.pages.k, next);
+                if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait_bounded(&v_empty[st], ((i >> 1) - 1) & 1))) { ok = false; break; }
+                store(smem + S::v_off + st * 32768, rv);
+                fence_proxy_async_smem();
+                mbar_arrive(&v_full[st]);
+                row = next;
+            }
+        }
+        if (!ok && lane == 0 && p.err) atomicOr(p.err, ERR_WAIT_PREFILL);
+    } else if (warp == 8) {
+        // ---- products --------------------------------------------------------------------------------
+        if (lane == 0) {
+            const int nb[2] = {half_blocks(0), half_blocks(1)};
+            const uint32_t id_s = pc_idesc<T>(false), id_o = pc_idesc<T>(true);
+            bool ok = mbar_wait_bounded(q_full, 0);
+            tc_fence_after();
+            auto scores = [&](int hf, int i) {
+                const uint64_t qd = umma_desc_sw128(smem_u32(smem + S::q_off + hf * 32768));
+                const uint64_t kd = umma_desc_sw128(smem_u32(smem + S::k_off + (i & 1) * 32768));
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) {
+                    const int off = (ks >> 2) * 1024 + 2 * (ks & 3);
+                    tc_mma_f16(tmem + 128 * hf, qd + off, kd + off, id_s, ks != 0);
+                }
+                tc_commit(&s_full[hf]);
+            };
+            if (ok && nblk > 0) {
+                ok = mbar_wait_bounded(&k_full[0], 0);
+                tc_fence_after();
+                if (ok) {
+                    for (int hf = 0; hf < 2; ++hf)
+                        if (nb[hf] > 0) scores(hf, 0);
+                    tc_commit(&k_empty[0]);
+                }
+            }
+            for (int i = 0; ok && i < nblk; ++i) {
+                const int st = i & 1;
+                if (!(ok = mbar_wait_bounded(&v_full[st], (i >> 1) & 1))) break;
+                if (i + 1 < nblk && !(ok = mbar_wait_bounded(&k_full[(i + 1) & 1], ((i + 1) >> 1) & 1))) break;
+                for (int hf = 0; ok && hf < 2; ++hf) {
+                    if (i >= nb[hf]) continue;
+                    if (!(ok = mbar_wait_bounded(&p_full[hf], i & 1))) break;
+                    tc_fence_after();
+                    const uint64_t vd = umma_desc_sw128_mn(smem_u32(smem + S::v_off + st * 32768), 16384);
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks)
+                        tc_mma_f16_ts(tmem + 256 + 128 * hf, tmem + 128 * hf + 8 * ks, vd + 128 * ks, id_o, (i | ks) != 0);
+                    if (i + 1 < nb[hf]) scores(hf, i + 1);
+                    else tc_commit(&o_full[hf]);
+                }
+                if (!ok) break;
+                tc_commit(&v_empty[st]);
+                if (i + 1 < nblk) tc_commit(&k_empty[(i + 1) & 1]);
+            }
+            if (!ok && p.err) atomicOr(p.err, ERR_WAIT_PREFILL);
+            tc_commit(done);  // every product issued has completed before tensor memory is freed
+            mbar_wait_bounded(done, 0);
+        }
+    } else {
+        // ---- softmax ---------------------------------------------------------------------------------
+        const int hf = warp >> 2, quarter = warp & 3;
+        const int R = t.row0 + 128 * hf + 32 * quarter + lane;
+        const int lim = R < rows ? t.kv - t.n + R / G : -1;
+        const int nb = half_blocks(hf);
+        const uint32_t s_tm = tmem + 128 * hf + ((uint32_t)(32 * quarter) << 16), o_tm = s_tm + 256;
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int i = 0; i < nb; ++i) {
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&s_full[hf], i & 1))) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const int k0 = (t.j0 + i) * PC_BK;
+            const bool edge = __any_sync(0xffffffffu, lim < k0 + PC_BK - 1);
+            const float* f = reinterpret_cast<const float*>(smem + S::c_off) + (i & 3) * 384;
+            if (Q8 && !__all_sync(0xffffffffu, mbar_wait_bounded(&c_full[i & 3], (i >> 2) & 1))) {
+                ok = false;
+                break;
+            }
+            // this row's score of key c of the block, in units of log2
+            auto score = [&](float s, int c) {
+                s = Q8 ? fmaf(s, f[c], f[128 + c]) : s * p.scale_log2;
+                return edge && k0 + c > lim ? -INFINITY : s;
+            };
+            float bm = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float v[64];
+                tmem_ld64(s_tm + 64 * c, v);
+#pragma unroll
+                for (int e = 0; e < 64; ++e) bm = fmaxf(bm, score(v[e], 64 * c + e));
+            }
+            const bool move = bm > m + 8.f;  // (from -inf: any finite score)
+            if (__any_sync(0xffffffffu, move)) {
+                const float corr = move ? (m == -INFINITY ? 0.f : exp2f(m - bm)) : 1.f;
+                if (move) m = bm;
+                l *= corr;
+                if (i > 0) {  // (O is complete up to the block before: S of this one was issued after it)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float v[32];
+                        tmem_ld32(o_tm + 32 * c, v);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] *= corr;
+                        tmem_st32(o_tm + 32 * c, v);
+                    }
+                }
+            }
+            const float ms = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float v[64];
+                tmem_ld64(s_tm + 64 * c, v);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    uint32_t r[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int x = 64 * c + 32 * b + 2 * e;
+                        const float e0 = ex2_approx(score(v[32 * b + 2 * e], x) - ms);
+                        const float e1 = ex2_approx(score(v[32 * b + 2 * e + 1], x + 1) - ms);
+                        l += Q8 ? fmaf(e0, f[256 + x], e1 * f[257 + x]) : e0 + e1;
+                        r[e] = pack_f<T>(e0, e1);
+                    }
+                    tmem_st16(s_tm + 32 * c + 16 * b, r);
+                }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[hf]);
+        }
+        if (ok && nb > 0 && !__all_sync(0xffffffffu, mbar_wait_bounded(&o_full[hf], 0))) ok = false;
+        tc_fence_after();
+        if (!ok) {
+            if (lane == 0 && p.err) atomicOr(p.err, ERR_WAIT_PREFILL);
+        } else {
+            const bool real = R < rows;
+            const float il = p.n_split > 1 ? 1.f : m == -INFINITY ? 0.f : 1.0f / l;
+            const int Rc = min(R, rows - 1);
+            T* dst = reinterpret_cast<T*>(p.out) + (t.q0 + Rc / G) * p.out_stride + (h * G + Rc % G) * HD;
+            float* pt = p.part + (size_t)blockIdx.x * PC_PART;
+            const int rt = 128 * hf + 32 * quarter + lane;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float v[32];
+                if (nb > 0) tmem_ld32(o_tm + 32 * c, v);
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = nb > 0 && il != 0.f ? v[8 * b + e] * il : 0.f;
+                    if (real) {
+                        if (p.n_split > 1) store8<float>(pt + rt * HD + 32 * c + 8 * b, x);
+                        else store8<T>(dst + 32 * c + 8 * b, x);
+                    }
+                }
+            }
+            if (p.n_split > 1) {
+                pt[PC_ROWS * HD + rt] = m;
+                pt[PC_ROWS * HD + PC_ROWS + rt] = l;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, PC_TMEM_COLS);
+    }
+}
+
+// Folds the n_split parts of every row, in the order of the keys.  Grid: n_kv x tiles x 32, eight rows a CTA.
+template <typename T>
+__global__ void __launch_bounds__(256) paged_attn_tc_join_kernel(const PagedTcParams p) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n_kv = p.pages.n_kv, G = p.group;
+    const int rt = (blockIdx.x & 31) * 8 + warp, h = (blockIdx.x >> 5) % n_kv, y = (blockIdx.x >> 5) / n_kv;
+    PcTile t{};
+    const bool live = pc_find(p.seqs, p.pages.ps_shift, G, p.min_rows, y, lane, t, nullptr);
+    pdl_wait();
+    const int R = t.row0 + rt;
+    if (!live || R >= t.n * G) return;
+    float m = -INFINITY, l = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int z = 0; z < p.n_split; ++z) {
+        const float* pt = p.part + (size_t)(h + n_kv * (z + p.n_split * y)) * PC_PART;
+        const float pm = pt[PC_ROWS * HD + rt], pl = pt[PC_ROWS * HD + PC_ROWS + rt];
+        const float4 v = *reinterpret_cast<const float4*>(pt + rt * HD + 4 * lane);
+        const float mn = fmaxf(m, pm);
+        const float f0 = m == -INFINITY ? 0.f : exp2f(m - mn), f1 = pm == -INFINITY ? 0.f : exp2f(pm - mn);
+        m = mn;
+        l = l * f0 + pl * f1;
+        a.x = a.x * f0 + v.x * f1;
+        a.y = a.y * f0 + v.y * f1;
+        a.z = a.z * f0 + v.z * f1;
+        a.w = a.w * f0 + v.w * f1;
+    }
+    const float il = m == -INFINITY ? 0.f : 1.0f / l;
+    T* dst = reinterpret_cast<T*>(p.out) + (t.q0 + R / G) * p.out_stride + (h * G + R % G) * HD + 4 * lane;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f<T>(a.x * il, a.y * il), pack_f<T>(a.z * il, a.w * il));
+}
+
+}  // namespace icua
