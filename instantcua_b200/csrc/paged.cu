@@ -153,25 +153,36 @@ bool q_type_fits(int dtype, int kvd) {
     return (dtype == ICUA_DT_F16 && kvd != ICUA_KV_BF16) || (dtype == ICUA_DT_BF16 && kvd != ICUA_KV_F16);
 }
 
-template <typename T, bool Q8>
+template <typename T, bool Q8, int MT>
 cudaError_t launch_attn(const PagedAttnParams& p, int dev, cudaStream_t st) {
-    const int smem = pa_smem(Q8);
-    cudaError_t e = allow_smem<paged_attn_kernel<T, Q8>>(smem, dev);
+    const int smem = pa_smem(Q8, MT);
+    cudaError_t e = allow_smem<paged_attn_kernel<T, Q8, MT>>(smem, dev);
     if (e != cudaSuccess) return e;
     const int ctas = std::min(PA_MAX_CTAS, 2 * sm_count(dev));
-    paged_attn_kernel<T, Q8><<<ctas, PA_THREADS, smem, st>>>(p);
+    paged_attn_kernel<T, Q8, MT><<<ctas, PA_THREADS, smem, st>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(PA_THREADS);
+    cfg.blockDim = dim3(512);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<T, pa_block(Q8)>, p, ctas);
+    return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<T, 16 * MT, pa_block(Q8)>, p, ctas);
 }
+
+template <int MT>
+cudaError_t launch_attn_rows(const PagedAttnParams& p, bool f16, bool q8, int dev, cudaStream_t st) {
+    return q8    ? (f16 ? launch_attn<__half, true, MT>(p, dev, st) : launch_attn<__nv_bfloat16, true, MT>(p, dev, st))
+           : f16 ? launch_attn<__half, false, MT>(p, dev, st)
+                 : launch_attn<__nv_bfloat16, false, MT>(p, dev, st);
+}
+
+// Sequences with up to PA_ROWS_FEW query rows per kv head go through the warp-MMA kernel, more rows
+// through the tensor-core kernel.
+constexpr int PA_ROWS_FEW = 64;
 
 // Tiles of the tensor-core kernel: a bound from what the host knows, and the shares of the keys that fill
 // the SMs when the tiles alone do not (two blocks of keys per share at least).
@@ -215,7 +226,7 @@ icua_status check_attn(const icua_kv_pages* pages, const icua_kv_seqs* seqs, int
     if (n_q < pages->n_kv || n_q > 256 || n_q % pages->n_kv) return bad("n_q %d is not a multiple of n_kv %d up to 256", n_q, pages->n_kv);
     // the kernels count blocks of keys over all items in 32 bits
     const int64_t rows = (int64_t)seqs->total_q * (n_q / pages->n_kv);
-    const double blocks = ((double)rows / PA_ROWS + seqs->n_seqs) * pages->n_kv * ((double)seqs->max_pages * pages->page_size / 64 + 1);
+    const double blocks = ((double)rows / 16 + seqs->n_seqs) * pages->n_kv * ((double)seqs->max_pages * pages->page_size / 64 + 1);
     if (rows > INT32_MAX || blocks > 4e9) return bad("the batch is too large: split it");
     return ICUA_OK;
 }
@@ -292,7 +303,7 @@ uint64_t icua_attn_paged_scratch_bytes(const icua_kv_pages* pages, const icua_kv
     PagesView P;
     SeqsView S;
     if (check_attn(pages, seqs, n_q, &P, &S) != ICUA_OK) return 0;
-    return PA_SCRATCH + ((int64_t)seqs->max_q * (n_q / pages->n_kv) > PA_ROWS ? PC_SCRATCH : 0);
+    return PA_SCRATCH + ((int64_t)seqs->max_q * (n_q / pages->n_kv) > PA_ROWS_FEW ? PC_SCRATCH : 0);
 }
 
 icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs, const icua_attn_paged_args* a, int32_t* err_dev,
@@ -319,15 +330,13 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
     p.n_q = a->n_q;
     p.group = a->n_q / pages->n_kv;
     p.scale_log2 = (a->scale > 0.f ? a->scale : 0.08838834764831845f) * 1.4426950408889634f;
-    p.max_rows = PA_ROWS;
+    p.max_rows = PA_ROWS_FEW;
     p.part = (float*)a->scratch;
     p.err = err_dev;
     cudaStream_t s = (cudaStream_t)stream;
     const bool f16 = a->dtype == ICUA_DT_F16, q8 = pages->dtype == ICUA_KV_Q8;
     cudaError_t e = cudaSuccess;
-    // Sequences of up to 16 query rows per kv head go through the warp-MMA kernel, which reads the cache
-    // at HBM speed whatever the rows; more rows through the tensor-core kernel.
-    const bool tc = (int64_t)seqs->max_q * p.group > PA_ROWS;
+    const bool tc = (int64_t)seqs->max_q * p.group > PA_ROWS_FEW;
     // A batch whose sequences all seem to bring max_q tokens goes there whole, one launch less (a shorter
     // sequence that it holds all the same is then a tile like any other).
     const bool all_tc = tc && (int64_t)seqs->n_seqs * seqs->max_q == seqs->total_q;
@@ -341,7 +350,7 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
         c.out_stride = p.out_stride;
         c.group = p.group;
         c.scale_log2 = p.scale_log2;
-        c.min_rows = all_tc ? 0 : PA_ROWS;
+        c.min_rows = all_tc ? 0 : PA_ROWS_FEW;
         c.part = (float*)((uint8_t*)a->scratch + PA_SCRATCH);
         c.err = err_dev;
         const TcGrid g = tc_grid(seqs, pages->n_kv, p.group, c.min_rows, sm_count(dev));
@@ -353,9 +362,7 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
     }
     p.alone = !tc;
     if (e == cudaSuccess && !all_tc)
-        e = q8 ? (f16 ? launch_attn<__half, true>(p, dev, s) : launch_attn<__nv_bfloat16, true>(p, dev, s))
-            : f16 ? launch_attn<__half, false>(p, dev, s)
-                  : launch_attn<__nv_bfloat16, false>(p, dev, s);
+        e = (int64_t)seqs->max_q * p.group > 16 ? launch_attn_rows<2>(p, f16, q8, dev, s) : launch_attn_rows<1>(p, f16, q8, dev, s);
     return e == cudaSuccess ? ICUA_OK : cuda_fail("icua_attn_paged", e);
 }
 

@@ -28,13 +28,13 @@
 
 namespace icua {
 
-constexpr int PA_ROWS = 16;       // query rows per item
+constexpr int PA_ROWS_MAX = 32;   // query rows per item: 16 or 32
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = PA_WARPS * 32;
 constexpr int PA_NS = 3;          // ring slots per warp
 constexpr int PA_MAX_CTAS = 320;  // workspace slots are laid out for so many
 constexpr int PA_MAX_SEQS = 1024;
-constexpr int PA_PART = PA_ROWS * HD + 2 * PA_ROWS;  // floats of a part: o[16][128], m[16], l[16]
+constexpr int PA_PART = PA_ROWS_MAX * HD + 2 * PA_ROWS_MAX;  // floats of a part: o[32][128], m[32], l[32]
 
 struct PagedAttnParams {
     PagesView pages;
@@ -53,7 +53,9 @@ struct PagedAttnParams {
 constexpr int pa_keys(bool q8) { return q8 ? 32 : 16; }  // rows of a warp's slot
 constexpr int pa_block(bool q8) { return PA_WARPS * pa_keys(q8); }
 constexpr int pa_slot(bool q8) { return q8 ? 32 * 2 * HD + 2 * 32 * 4 : 16 * 2 * HD * 2; }
-constexpr int pa_smem(bool q8) { return PA_WARPS * PA_NS * pa_slot(q8) + (PA_MAX_SEQS + 1) * 4; }
+constexpr int pa_smem(bool q8, int mt) {
+    return PA_WARPS * PA_NS * pa_slot(q8) + (mt > 1 ? mt * 16 * 2 * HD : 0) + (PA_MAX_SEQS + 1) * 4;
+}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
@@ -82,6 +84,17 @@ __device__ __forceinline__ uint32_t codes_to_pair<__nv_bfloat16>(uint32_t w) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+__device__ __forceinline__ float lg2_approx(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
     uint32_t r;
     asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
@@ -92,13 +105,13 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
 struct PaWork {
     int n, kv, q0, tiles, nb, items;
 };
-__device__ __forceinline__ PaWork pa_work(const SeqsView& S, int ps_shift, int n_kv, int group, int max_rows, int block, int s,
-                                          int* err, bool alone = false) {
+__device__ __forceinline__ PaWork pa_work(const SeqsView& S, int ps_shift, int n_kv, int group, int max_rows, int tile_rows,
+                                          int block, int s, int* err, bool alone = false) {
     const SeqInfo q = load_seq(S, ps_shift, s, err);
     PaWork w{q.n, q.kv, q.q0, 0, 0, 0};
     const long long rows = (long long)q.n * group;
     if (rows > 0 && rows <= max_rows) {
-        w.tiles = (int)((rows + PA_ROWS - 1) / PA_ROWS);
+        w.tiles = (int)((rows + tile_rows - 1) / tile_rows);
         w.items = w.tiles * n_kv;
         w.nb = max(1, (q.kv + block - 1) / block);  // an item without keys still writes its (zero) rows
     } else if (rows > 0 && alone && err) {
@@ -109,15 +122,15 @@ __device__ __forceinline__ PaWork pa_work(const SeqsView& S, int ps_shift, int n
 
 // pre[s] = blocks before sequence s, pre[n_seqs] = all of them.  `warp_tot` holds one word per warp.
 template <int THREADS>
-__device__ __forceinline__ uint32_t pa_prefix(const SeqsView& S, int ps_shift, int n_kv, int group, int max_rows, int block,
-                                              uint32_t* pre, uint32_t* warp_tot, int* err, bool alone = false) {
+__device__ __forceinline__ uint32_t pa_prefix(const SeqsView& S, int ps_shift, int n_kv, int group, int max_rows, int tile_rows,
+                                              int block, uint32_t* pre, uint32_t* warp_tot, int* err, bool alone = false) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint32_t base = 0;
     for (int s0 = 0; s0 < S.n_seqs; s0 += THREADS) {
         const int s = s0 + tid;
         uint32_t w = 0;
         if (s < S.n_seqs) {
-            const PaWork k = pa_work(S, ps_shift, n_kv, group, max_rows, block, s, err, alone);
+            const PaWork k = pa_work(S, ps_shift, n_kv, group, max_rows, tile_rows, block, s, err, alone);
             w = (uint32_t)k.items * (uint32_t)k.nb;
         }
         uint32_t x = w;
@@ -165,19 +178,20 @@ struct PaDeal {
     }
 };
 
-template <typename T, bool Q8>
+// MT: tiles of sixteen query rows per item that share every K and V fragment.
+template <typename T, bool Q8, int MT>
 __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAttnParams p) {
-    constexpr int KEYS = pa_keys(Q8), BLOCK = pa_block(Q8), SLOT = pa_slot(Q8);
+    constexpr int KEYS = pa_keys(Q8), BLOCK = pa_block(Q8), SLOT = pa_slot(Q8), NT = KEYS / 8, ROWS = 16 * MT;
     constexpr int ROW = Q8 ? HD : 2 * HD;  // bytes of a cached row
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ float ml[PA_WARPS][2][PA_ROWS];
+    __shared__ float ml[PA_WARPS][2][ROWS];
     __shared__ uint32_t warp_tot[PA_WARPS];
-    uint32_t* pre = reinterpret_cast<uint32_t*>(smem + PA_WARPS * PA_NS * SLOT);
+    uint8_t* q_tile = smem + PA_WARPS * PA_NS * SLOT;  // MT > 1: the rows of the item, 256 B each, chunk c at c ^ (row & 7)
+    uint32_t* pre = reinterpret_cast<uint32_t*>(q_tile + (MT > 1 ? ROWS * 2 * HD : 0));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int ps_shift = p.pages.ps_shift, n_kv = p.pages.n_kv, G = p.group;
-    const uint32_t total =
-        pa_prefix<PA_THREADS>(p.seqs, ps_shift, n_kv, G, p.max_rows, BLOCK, pre, warp_tot, blockIdx.x == 0 ? p.err : nullptr,
-                               p.alone != 0);
+    const uint32_t total = pa_prefix<PA_THREADS>(p.seqs, ps_shift, n_kv, G, p.max_rows, ROWS, BLOCK, pre, warp_tot,
+                                                 blockIdx.x == 0 ? p.err : nullptr, p.alone != 0);
     const PaDeal deal(total, gridDim.x);
     const uint32_t x0 = deal.begin(blockIdx.x), x1 = deal.begin(blockIdx.x + 1);
     pdl_launch_dependents();
@@ -190,7 +204,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
     auto at = [&](uint32_t x) {
         Cursor c;
         c.s = pa_find(pre, p.seqs.n_seqs, x);
-        c.w = pa_work(p.seqs, ps_shift, n_kv, G, p.max_rows, BLOCK, c.s, nullptr);
+        c.w = pa_work(p.seqs, ps_shift, n_kv, G, p.max_rows, ROWS, BLOCK, c.s, nullptr);
         const uint32_t y = x - pre[c.s];
         c.item = (int)(y / (uint32_t)c.w.nb);
         c.b = (int)(y % (uint32_t)c.w.nb);
@@ -203,7 +217,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
             do {
                 ++c.s;
             } while (pre[c.s + 1] == pre[c.s]);
-            c.w = pa_work(p.seqs, ps_shift, n_kv, G, p.max_rows, BLOCK, c.s, nullptr);
+            c.w = pa_work(p.seqs, ps_shift, n_kv, G, p.max_rows, ROWS, BLOCK, c.s, nullptr);
         }
     };
 
@@ -271,55 +285,88 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
     while (x < x1) {
         const int h = c.item / c.w.tiles, tile = c.item - h * c.w.tiles;
         const int b0 = c.b, b1 = (int)min((uint32_t)c.w.nb, c.b + (x1 - x));
-        // this lane's rows g and g + 8: query pointers and last visible positions
+        // this lane's rows g and g + 8 of every sixteen: last visible positions
         const int rows = c.w.n * G;
-        const T* qp[2];
-        int lim[2];
+        auto q_row = [&](int r) {  // row r of the item (rows past the end: the last one, never stored)
+            const int rr = min(tile * ROWS + r, rows - 1);
+            return reinterpret_cast<const T*>(p.q) + (c.w.q0 + rr / G) * p.q_stride + (h * G + rr % G) * HD;
+        };
+        int lim[MT][2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = tile * PA_ROWS + g + 8 * i;
-            const int tok = min(r, rows - 1) / G, hd = min(r, rows - 1) % G;
-            qp[i] = reinterpret_cast<const T*>(p.q) + (c.w.q0 + tok) * p.q_stride + (h * G + hd) * HD;
-            lim[i] = r < rows ? c.w.kv - c.w.n + tok : -1;
-        }
-        uint32_t qa[8][4];
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-            if (!Q8) {
+            for (int i = 0; i < 2; ++i) {
+                const int r = tile * ROWS + 16 * mt + g + 8 * i;
+                lim[mt][i] = r < rows ? c.w.kv - c.w.n + r / G : -1;
+            }
+        // A fragments of q.  In a q8 cache a lane's K codes are 32-bit words of four dimensions d0 .. d0 + 3, used
+        // as the pairs (d0, d0 + 2) and (d0 + 1, d0 + 3), so q takes the same order: word 2 t + 16 ks of a row
+        // holds the first pair of d0 = 64 (ks / 4) + 16 t + 4 (ks % 4), word 2 t + 16 ks + 8 the second.
+        uint32_t qa[MT == 1 ? 8 : 1][4];
+        if (MT == 1) {
+            const T* qp[2] = {q_row(g), q_row(g + 8)};
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    qa[ks][i] = *reinterpret_cast<const uint32_t*>(qp[i] + 16 * ks + 2 * t);
-                    qa[ks][2 + i] = *reinterpret_cast<const uint32_t*>(qp[i] + 16 * ks + 2 * t + 8);
+                    if (!Q8) {
+                        qa[ks][i] = *reinterpret_cast<const uint32_t*>(qp[i] + 16 * ks + 2 * t);
+                        qa[ks][2 + i] = *reinterpret_cast<const uint32_t*>(qp[i] + 16 * ks + 2 * t + 8);
+                    } else {
+                        const uint2 v = *reinterpret_cast<const uint2*>(qp[i] + 64 * (ks >> 2) + 16 * t + 4 * (ks & 3));
+                        qa[ks][i] = prmt(v.x, v.y, 0x5410);
+                        qa[ks][2 + i] = prmt(v.x, v.y, 0x7632);
+                    }
                 }
-            } else {
-                // a lane's K codes are 32-bit words of four dimensions d0 .. d0 + 3, used as (d0, d0 + 2) and
-                // (d0 + 1, d0 + 3): the same order here
-                const int d0 = (ks < 4 ? 0 : 64) + 16 * t + 4 * (ks & 3);
+        } else {
+            // (the barriers at the end of an item are behind every read of the tile before)
+            for (int e = tid; e < ROWS * 16; e += PA_THREADS) {
+                const int r = e >> 4, ch = e & 15;
+                const uint4 v = *reinterpret_cast<const uint4*>(q_row(r) + 8 * ch);
+                if (!Q8) {
+                    *reinterpret_cast<uint4*>(q_tile + r * 256 + ((ch ^ (r & 7)) << 4)) = v;
+                } else {
+                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint2 v = *reinterpret_cast<const uint2*>(qp[i] + d0);
-                    qa[ks][i] = prmt(v.x, v.y, 0x5410);
-                    qa[ks][2 + i] = prmt(v.x, v.y, 0x7632);
+                    for (int f = 0; f < 2; ++f) {  // dimensions 8 ch + 4 f ..
+                        const int d = 8 * ch + 4 * f, ks = 4 * (d >> 6) + ((d >> 2) & 3), tt = (d >> 4) & 3;
+                        uint8_t* qr = q_tile + r * 256 + 4 * tt;
+                        *reinterpret_cast<uint32_t*>(qr + (((2 * ks) ^ (r & 7)) << 4)) = prmt(w[2 * f], w[2 * f + 1], 0x5410);
+                        *reinterpret_cast<uint32_t*>(qr + (((2 * ks + 1) ^ (r & 7)) << 4)) = prmt(w[2 * f], w[2 * f + 1], 0x7632);
+                    }
                 }
             }
+            __syncthreads();
         }
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-        float o[16][4];
+        const uint32_t q_u = smem_u32(q_tile);
+        auto q_frag = [&](int mt, int ks, uint32_t (&a)[4]) {
+            if (MT == 1) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
+                for (int i = 0; i < 4; ++i) a[i] = qa[MT == 1 ? ks : 0][i];
+            } else {  // rows 0-7 / 8-15 of chunk 2 ks, then of 2 ks + 1
+                const int r = 16 * mt + (lane & 15);
+                ldsm_x4(a, q_u + r * 256 + (((2 * ks + (lane >> 4)) ^ (r & 7)) << 4));
+            }
+        };
+        float m[MT][2], l[MT][2], o[MT][16][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[j][i] = 0.f;
+        for (int mt = 0; mt < MT; ++mt) {
+            m[mt][0] = m[mt][1] = -INFINITY;
+            l[mt][0] = l[mt][1] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[mt][j][i] = 0.f;
+        }
 
         for (int b = b0; b < b1; ++b) {
             cp_async_wait<PA_NS - 1>();
             __syncwarp();
             const uint32_t sk = ring_u + slot * SLOT, sv = sk + KEYS * ROW;
             const uint8_t* sp = ring + slot * SLOT;
-#pragma unroll
-            for (int part = 0; part < KEYS / 16; ++part) {
-                const int k0 = b * BLOCK + warp * KEYS + 16 * part;
-                if (k0 >= c.w.kv || (dead >> (slot * 2 + part)) & 1) continue;
-                float s[2][4] = {};
+            const int k0 = b * BLOCK + warp * KEYS;
+            if (k0 < c.w.kv) {
+                float s[MT][NT][4] = {};
                 if (!Q8) {
                     // matrices: keys 0-7 / dims 0-7, keys 0-7 / dims 8-15, keys 8-15 / ...
                     const int row = (lane & 7) + ((lane >> 4) << 3);
@@ -327,30 +374,41 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
                     for (int ks = 0; ks < 8; ++ks) {
                         uint32_t kb[4];
                         ldsm_x4(kb, sk + row * ROW + (((2 * ks + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
-                        mma_kv<T>(s[0], qa[ks], kb[0], kb[1]);
-                        mma_kv<T>(s[1], qa[ks], kb[2], kb[3]);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            uint32_t a[4];
+                            q_frag(mt, ks, a);
+                            mma_kv<T>(s[mt][0], a, kb[0], kb[1]);
+                            mma_kv<T>(s[mt][1], a, kb[2], kb[3]);
+                        }
                     }
                 } else {
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
-                        const int r = 8 * nt + g;
+                    for (int half = 0; half < 2; ++half) {
+                        uint4 w4[NT];
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(sp + (16 * part + r) * ROW +
-                                                                            (((t + 4 * half) ^ ((r & 1) << 2)) << 4));
-                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                        for (int nt = 0; nt < NT; ++nt)
+                            w4[nt] = *reinterpret_cast<const uint4*>(sp + (8 * nt + g) * ROW + (((t + 4 * half) ^ ((g & 1) << 2)) << 4));
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                mma_kv<T>(s[nt], qa[4 * half + i], codes_to_pair<T>(w[i]), codes_to_pair<T>(w[i] >> 8));
-                        }
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) {
+                                uint32_t a[4];
+                                q_frag(mt, 4 * half + i, a);
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    const uint32_t w = i == 0 ? w4[nt].x : i == 1 ? w4[nt].y : i == 2 ? w4[nt].z : w4[nt].w;
+                                    mma_kv<T>(s[mt][nt], a, codes_to_pair<T>(w), codes_to_pair<T>(w >> 8));
+                                }
+                            }
                     }
                 }
-                // columns of this lane: keys 2t, 2t + 1, 2t + 8, 2t + 9
-                float inv[4];
+                // columns of this lane: keys 8 nt + 2t, + 1
+                float inv[2 * NT];
                 if (Q8) {
-                    const float* kscale = reinterpret_cast<const float*>(sp + 2 * KEYS * ROW) + 16 * part;
+                    const float* kscale = reinterpret_cast<const float*>(sp + 2 * KEYS * ROW);
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
+                    for (int nt = 0; nt < NT; ++nt) {
                         const float2 a = *reinterpret_cast<const float2*>(kscale + 8 * nt + 2 * t);
                         const float2 v = *reinterpret_cast<const float2*>(kscale + KEYS + 8 * nt + 2 * t);
                         const float av[2] = {a.x, a.y}, vv[2] = {v.x, v.y};
@@ -359,56 +417,66 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
                             // a NaN scale (a poisoned row) reaches the rows that see it through the score; a masked
                             // one adds 0 x 0 to their sums
                             const float vs = vv[e] < 1e-37f ? 1e-37f : vv[e];
-                            const float add = log2f(vs), mul = av[e] * p.scale_log2;
-                            inv[2 * nt + e] = vs == vs ? 1.0f / vs : 0.f;
-                            s[nt][e] = fmaf(s[nt][e], mul, add);
-                            s[nt][2 + e] = fmaf(s[nt][2 + e], mul, add);
+                            const float add = lg2_approx(vs), mul = av[e] * p.scale_log2;
+                            inv[2 * nt + e] = vs == vs ? rcp_approx(vs) : 0.f;
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) {
+                                s[mt][nt][e] = fmaf(s[mt][nt][e], mul, add);
+                                s[mt][nt][2 + e] = fmaf(s[mt][nt][2 + e], mul, add);
+                            }
                         }
                     }
                 } else {
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt)
+                    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[nt][e] *= p.scale_log2;
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[mt][nt][e] *= p.scale_log2;
                 }
-                float mn[2];
+                uint32_t pa[MT][NT / 2][4];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float bm = -INFINITY;
+                for (int mt = 0; mt < MT; ++mt) {
+                    const uint32_t gone = dead >> (2 * slot);
+                    if (gone & 3u || __any_sync(0xffffffffu, k0 + KEYS - 1 > min(lim[mt][0], lim[mt][1]))) {
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt)
+                        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float& v = s[nt][2 * i + e];
-                            v = k0 + 8 * nt + 2 * t + e <= lim[i] ? v : -INFINITY;
-                            bm = fmaxf(bm, v);
-                        }
-                    bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
-                    bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
-                    mn[i] = fmaxf(m[i], bm);
-                }
-                if (__any_sync(0xffffffffu, mn[0] > m[0] || mn[1] > m[1])) {
+                            for (int e = 0; e < 4; ++e)
+                                if (k0 + 8 * nt + 2 * t + (e & 1) > lim[mt][e >> 1] || (gone >> (nt >> 1)) & 1u) s[mt][nt][e] = -INFINITY;
+                    }
+                    float mn[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float corr = m[i] == -INFINITY ? 0.f : exp2f(m[i] - mn[i]);
-                        m[i] = mn[i];
-                        l[i] *= corr;
+                        float bm = fmaxf(s[mt][0][2 * i], s[mt][0][2 * i + 1]);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            o[j][2 * i] *= corr;
-                            o[j][2 * i + 1] *= corr;
+                        for (int nt = 1; nt < NT; ++nt) bm = fmaxf(bm, fmaxf(s[mt][nt][2 * i], s[mt][nt][2 * i + 1]));
+                        bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
+                        bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
+                        mn[i] = fmaxf(m[mt][i], bm);
+                    }
+                    if (__any_sync(0xffffffffu, mn[0] > m[mt][0] || mn[1] > m[mt][1])) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float corr = m[mt][i] == -INFINITY ? 0.f : ex2_approx(m[mt][i] - mn[i]);
+                            m[mt][i] = mn[i];
+                            l[mt][i] *= corr;
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                o[mt][j][2 * i] *= corr;
+                                o[mt][j][2 * i + 1] *= corr;
+                            }
                         }
                     }
-                }
-                uint32_t pa[4];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float ms = m[i] == -INFINITY ? 0.f : m[i];
+                    for (int i = 0; i < 2; ++i) {
+                        const float ms = m[mt][i] == -INFINITY ? 0.f : m[mt][i];
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
-                        const float e0 = ex2_approx(s[nt][2 * i] - ms), e1 = ex2_approx(s[nt][2 * i + 1] - ms);
-                        l[i] += Q8 ? fmaf(e0, inv[2 * nt], e1 * inv[2 * nt + 1]) : e0 + e1;
-                        pa[2 * nt + i] = pack_f<T>(e0, e1);
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const float e0 = ex2_approx(s[mt][nt][2 * i] - ms), e1 = ex2_approx(s[mt][nt][2 * i + 1] - ms);
+                            l[mt][i] += Q8 ? fmaf(e0, inv[2 * nt], e1 * inv[2 * nt + 1]) : e0 + e1;
+                            pa[mt][nt >> 1][2 * (nt & 1) + i] = pack_f<T>(e0, e1);
+                        }
                     }
                 }
                 if (!Q8) {
@@ -417,24 +485,32 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
                     for (int j = 0; j < 8; ++j) {
                         uint32_t vb[4];  // keys 0-7 / 8-15 of dims 16j .. 16j + 7, then of 16j + 8 ..
                         ldsm_x4_trans(vb, sv + row * ROW + (((2 * j + (lane >> 4)) ^ (row & 7)) << 4));
-                        mma_kv<T>(o[2 * j], pa, vb[0], vb[1]);
-                        mma_kv<T>(o[2 * j + 1], pa, vb[2], vb[3]);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            mma_kv<T>(o[mt][2 * j], pa[mt][0], vb[0], vb[1]);
+                            mma_kv<T>(o[mt][2 * j + 1], pa[mt][0], vb[2], vb[3]);
+                        }
                     }
                 } else {
                     // column n of product j is dimension 16 n + j: lane g's chunk of a row holds all sixteen
-                    uint32_t w[4][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = 2 * t + (i & 1) + 8 * (i >> 1);
-                        const uint4 v = *reinterpret_cast<const uint4*>(sp + KEYS * ROW + (16 * part + r) * ROW +
-                                                                        ((g ^ (((r >> 1) & 3) << 1)) << 4));
-                        w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
-                    }
+                    for (int part = 0; part < NT / 2; ++part) {
+                        uint32_t w[4][4];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const uint32_t sel = 0x0040 << 4 | (j & 3) << 8 | (j & 3);  // bytes j of the two keys
-                        mma_kv<T>(o[j], pa, codes_to_pair<T>(prmt(w[0][j >> 2], w[1][j >> 2], sel)),
-                                  codes_to_pair<T>(prmt(w[2][j >> 2], w[3][j >> 2], sel)));
+                        for (int i = 0; i < 4; ++i) {
+                            const int r = 2 * t + (i & 1) + 8 * (i >> 1);
+                            const uint4 v = *reinterpret_cast<const uint4*>(sp + KEYS * ROW + (16 * part + r) * ROW +
+                                                                            ((g ^ (((r >> 1) & 3) << 1)) << 4));
+                            w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const uint32_t sel = 0x0400 | (j & 3) << 8 | (j & 3);  // byte j of the two keys
+                            const uint32_t b0 = codes_to_pair<T>(prmt(w[0][j >> 2], w[1][j >> 2], sel));
+                            const uint32_t b1 = codes_to_pair<T>(prmt(w[2][j >> 2], w[3][j >> 2], sel));
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) mma_kv<T>(o[mt][j], pa[mt][part], b0, b1);
+                        }
                     }
                 }
             }
@@ -444,82 +520,87 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
                 slot = slot + 1 == PA_NS ? 0 : slot + 1;
             }
         }
-        // the end of the item, or of this CTA's share of it: the warps meet in the slots they have just
-        // used up ([16][128] fp32 each; float4 column c4 of row r at c4 ^ 2 ((c4 >> 3) & 3) ^ (r & 1))
+        // the end of the item, or of this CTA's share of it: sixteen rows at a time the warps meet in the
+        // slots they have just used up ([16][128] fp32 each; float4 column c4 of row r at
+        // c4 ^ 2 ((c4 >> 3) & 3) ^ (r & 1))
         float* mine = reinterpret_cast<float*>(ring + slot * SLOT);
+        const bool whole = b0 == 0 && b1 == c.w.nb;
+        float* pt = p.part + (size_t)(2 * blockIdx.x + (b0 == 0 ? 1 : 0)) * PA_PART;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-            if (t == 0) {
-                ml[warp][0][g + 8 * i] = m[i];
-                ml[warp][1][g + 8 * i] = l[i];
-            }
-            const int r = g + 8 * i;
-            auto place = [&](int c4) { return mine + r * HD + 4 * (c4 ^ (((c4 >> 3) & 3) << 1) ^ (r & 1)); };
-            if (!Q8) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    *reinterpret_cast<float2*>(place(2 * j + (t >> 1)) + 2 * (t & 1)) = make_float2(o[j][2 * i], o[j][2 * i + 1]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        *reinterpret_cast<float4*>(place(8 * t + 4 * e + j)) =
-                            make_float4(o[4 * j][2 * i + e], o[4 * j + 1][2 * i + e], o[4 * j + 2][2 * i + e], o[4 * j + 3][2 * i + e]);
-            }
-        }
-        __syncthreads();
-        {
-            const int r = tid >> 3;  // eight threads a row, sixteen columns each
-            float mm = ml[0][0][r];
-#pragma unroll
-            for (int w = 1; w < PA_WARPS; ++w) mm = fmaxf(mm, ml[w][0][r]);
-            float fw[PA_WARPS], ll = 0.f;
-#pragma unroll
-            for (int w = 0; w < PA_WARPS; ++w) {
-                fw[w] = mm == -INFINITY ? 0.f : exp2f(ml[w][0][r] - mm);
-                ll = fmaf(fw[w], ml[w][1][r], ll);
-            }
-            const bool whole = b0 == 0 && b1 == c.w.nb;
-            const float il = mm == -INFINITY ? 0.f : 1.0f / ll;
-            const int rr = tile * PA_ROWS + r;
-            float* pt = p.part + (size_t)(2 * blockIdx.x + (b0 == 0 ? 1 : 0)) * PA_PART;
-            T* dst = reinterpret_cast<T*>(p.out) + (c.w.q0 + rr / G) * p.out_stride + (h * G + rr % G) * HD;
+        for (int mt = 0; mt < MT; ++mt) {
+            if (mt > 0) __syncthreads();
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int col = 8 * ((tid & 7) + 8 * i);
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int c4 = col / 4 + e;
-                    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                    for (int w = 0; w < PA_WARPS; ++w) {
-                        const float4 v = *reinterpret_cast<const float4*>(
-                            reinterpret_cast<const float*>(smem + (w * PA_NS + slot) * SLOT) + r * HD +
-                            4 * (c4 ^ (((c4 >> 3) & 3) << 1) ^ (r & 1)));
-                        a.x = fmaf(fw[w], v.x, a.x);
-                        a.y = fmaf(fw[w], v.y, a.y);
-                        a.z = fmaf(fw[w], v.z, a.z);
-                        a.w = fmaf(fw[w], v.w, a.w);
-                    }
-                    y[4 * e] = a.x; y[4 * e + 1] = a.y; y[4 * e + 2] = a.z; y[4 * e + 3] = a.w;
+                l[mt][i] += __shfl_xor_sync(0xffffffffu, l[mt][i], 1);
+                l[mt][i] += __shfl_xor_sync(0xffffffffu, l[mt][i], 2);
+                if (t == 0) {
+                    ml[warp][0][16 * mt + g + 8 * i] = m[mt][i];
+                    ml[warp][1][16 * mt + g + 8 * i] = l[mt][i];
                 }
-                if (rr < rows) {
+                const int r = g + 8 * i;
+                auto place = [&](int c4) { return mine + r * HD + 4 * (c4 ^ (((c4 >> 3) & 3) << 1) ^ (r & 1)); };
+                if (!Q8) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        *reinterpret_cast<float2*>(place(2 * j + (t >> 1)) + 2 * (t & 1)) =
+                            make_float2(o[mt][j][2 * i], o[mt][j][2 * i + 1]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            *reinterpret_cast<float4*>(place(8 * t + 4 * e + j)) =
+                                make_float4(o[mt][4 * j][2 * i + e], o[mt][4 * j + 1][2 * i + e], o[mt][4 * j + 2][2 * i + e],
+                                            o[mt][4 * j + 3][2 * i + e]);
+                }
+            }
+            __syncthreads();
+            const int r = tid >> 3, rt = 16 * mt + r;  // eight threads a row, sixteen columns each
+            const int rr = tile * ROWS + rt;
+            if (rr < rows) {
+                float mm = ml[0][0][rt];
+#pragma unroll
+                for (int w = 1; w < PA_WARPS; ++w) mm = fmaxf(mm, ml[w][0][rt]);
+                float fw[PA_WARPS], ll = 0.f;
+#pragma unroll
+                for (int w = 0; w < PA_WARPS; ++w) {
+                    fw[w] = mm == -INFINITY ? 0.f : ex2_approx(ml[w][0][rt] - mm);
+                    ll = fmaf(fw[w], ml[w][1][rt], ll);
+                }
+                const float il = mm == -INFINITY ? 0.f : 1.0f / ll;
+                T* dst = reinterpret_cast<T*>(p.out) + (c.w.q0 + rr / G) * p.out_stride + (h * G + rr % G) * HD;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int col = 8 * ((tid & 7) + 8 * i);
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int c4 = col / 4 + e;
+                        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                        for (int w = 0; w < PA_WARPS; ++w) {
+                            const float4 v = *reinterpret_cast<const float4*>(
+                                reinterpret_cast<const float*>(smem + (w * PA_NS + slot) * SLOT) + r * HD +
+                                4 * (c4 ^ (((c4 >> 3) & 3) << 1) ^ (r & 1)));
+                            a.x = fmaf(fw[w], v.x, a.x);
+                            a.y = fmaf(fw[w], v.y, a.y);
+                            a.z = fmaf(fw[w], v.z, a.z);
+                            a.w = fmaf(fw[w], v.w, a.w);
+                        }
+                        y[4 * e] = a.x; y[4 * e + 1] = a.y; y[4 * e + 2] = a.z; y[4 * e + 3] = a.w;
+                    }
                     if (whole) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) y[e] *= il;
                         store8<T>(dst + col, y);
                     } else {
-                        store8<float>(pt + r * HD + col, y);
+                        store8<float>(pt + rt * HD + col, y);
                     }
                 }
-            }
-            if (!whole && (tid & 7) == 0) {
-                pt[PA_ROWS * HD + r] = mm;
-                pt[PA_ROWS * HD + PA_ROWS + r] = ll;
+                if (!whole && (tid & 7) == 0) {
+                    pt[PA_ROWS_MAX * HD + rt] = mm;
+                    pt[PA_ROWS_MAX * HD + PA_ROWS_MAX + rt] = ll;
+                }
             }
         }
         __syncthreads();
@@ -532,46 +613,97 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
 }
 
 // Folds the parts of the items that more than one CTA of paged_attn_kernel (grid `ctas`, the same
-// arguments) worked on, in the order of their keys.  CTA c takes the item that c began and did not end.
-template <typename T, int BLOCK>
-__global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PagedAttnParams p, int ctas) {
+// arguments) worked on.  CTA c takes the item that c began and did not end.  Sixteen warps: with few rows
+// several warps share one (each takes every W-th part, eight in flight) and meet in shared memory; the
+// grouping depends on the sizes alone, so the bits do too.
+template <typename T, int ROWS, int BLOCK>
+__global__ void __launch_bounds__(512) paged_attn_join_kernel(const PagedAttnParams p, int ctas) {
     __shared__ uint32_t pre[PA_MAX_SEQS + 1];
-    __shared__ uint32_t warp_tot[PA_WARPS];
-    const int tid = threadIdx.x, G = p.group;
-    const uint32_t total = pa_prefix<PA_THREADS>(p.seqs, p.pages.ps_shift, p.pages.n_kv, G, p.max_rows, BLOCK, pre, warp_tot, nullptr);
+    __shared__ uint32_t warp_tot[16];
+    __shared__ float4 acc_s[16][32];
+    __shared__ float ml_s[16][2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.group;
+    const uint32_t total =
+        pa_prefix<512>(p.seqs, p.pages.ps_shift, p.pages.n_kv, G, p.max_rows, ROWS, BLOCK, pre, warp_tot, nullptr);
     const PaDeal deal(total, ctas);
     const uint32_t c0 = blockIdx.x, x0 = deal.begin(c0), x1 = deal.begin(c0 + 1);
     if (x0 >= x1) return;
     const int s = pa_find(pre, p.seqs.n_seqs, x1 - 1);
-    const PaWork w = pa_work(p.seqs, p.pages.ps_shift, p.pages.n_kv, G, p.max_rows, BLOCK, s, nullptr);
+    const PaWork w = pa_work(p.seqs, p.pages.ps_shift, p.pages.n_kv, G, p.max_rows, ROWS, BLOCK, s, nullptr);
     const uint32_t item = (x1 - 1 - pre[s]) / w.nb, i0 = pre[s] + item * w.nb, i1 = i0 + w.nb;
     if (i0 < x0 || i1 <= x1) return;
-    const uint32_t c1 = deal.cta_of(i1 - 1);
-    const int h = item / w.tiles, tile = item % w.tiles, rows = min(PA_ROWS, w.n * G - tile * PA_ROWS);
+    const int n_parts = (int)(deal.cta_of(i1 - 1) - c0) + 1;
+    const int h = item / w.tiles, tile = item % w.tiles, rows = min(ROWS, w.n * G - tile * ROWS);
+    int log_r = 0;  // rows in a round, a power of two up to 16; W = 16 >> log_r warps a row
+    while (log_r < 4 && (1 << log_r) < rows) ++log_r;
+    const int W = 16 >> log_r, piece = warp >> log_r;
     pdl_wait();
-    // thread = four columns of every fourth row
-    for (int r = tid >> 5; r < rows; r += PA_THREADS / 32) {
-        const int col = 4 * (tid & 31);
+    for (int r0 = 0; r0 < rows; r0 += 1 << log_r) {
+        const int r = r0 + (warp & ((1 << log_r) - 1));
         float m = -INFINITY, l = 0.f;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (uint32_t c = c0; c <= c1; ++c) {
-            const float* pt = p.part + (size_t)(2 * c + (c == c0 ? 1 : 0)) * PA_PART;
-            const float pm = pt[PA_ROWS * HD + r], pl = pt[PA_ROWS * HD + PA_ROWS + r];
-            const float4 v = *reinterpret_cast<const float4*>(pt + r * HD + col);
-            const float mn = fmaxf(m, pm);
-            const float f0 = m == -INFINITY ? 0.f : exp2f(m - mn), f1 = pm == -INFINITY ? 0.f : exp2f(pm - mn);
-            m = mn;
-            l = l * f0 + pl * f1;
-            a.x = a.x * f0 + v.x * f1;
-            a.y = a.y * f0 + v.y * f1;
-            a.z = a.z * f0 + v.z * f1;
-            a.w = a.w * f0 + v.w * f1;
+        if (r < rows) {
+            for (int k0 = piece; k0 < n_parts; k0 += 8 * W) {
+                float pm[8], pl[8];
+                float4 v[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int k = k0 + u * W;
+                    pm[u] = -INFINITY;
+                    if (k < n_parts) {
+                        const float* pt = p.part + (size_t)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * PA_PART;
+                        pm[u] = pt[PA_ROWS_MAX * HD + r];
+                        pl[u] = pt[PA_ROWS_MAX * HD + PA_ROWS_MAX + r];
+                        v[u] = *reinterpret_cast<const float4*>(pt + r * HD + 4 * lane);
+                    }
+                }
+                float mn = m;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) mn = fmaxf(mn, pm[u]);
+                const float f0 = m == -INFINITY ? 0.f : ex2_approx(m - mn);
+                m = mn;
+                l *= f0;
+                a.x *= f0; a.y *= f0; a.z *= f0; a.w *= f0;
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (pm[u] != -INFINITY) {
+                        const float f = ex2_approx(pm[u] - mn);
+                        l = fmaf(pl[u], f, l);
+                        a.x = fmaf(v[u].x, f, a.x);
+                        a.y = fmaf(v[u].y, f, a.y);
+                        a.z = fmaf(v[u].z, f, a.z);
+                        a.w = fmaf(v[u].w, f, a.w);
+                    }
+            }
         }
-        const float il = m == -INFINITY ? 0.f : 1.0f / l;
-        const int rr = tile * PA_ROWS + r;
-        T* dst = reinterpret_cast<T*>(p.out) + (w.q0 + rr / G) * p.out_stride + (h * G + rr % G) * HD + col;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f<T>(a.x * il, a.y * il), pack_f<T>(a.z * il, a.w * il));
+        if (W > 1) {
+            acc_s[warp][lane] = a;
+            if (lane == 0) {
+                ml_s[warp][0] = m;
+                ml_s[warp][1] = l;
+            }
+            __syncthreads();
+            if (piece == 0)
+                for (int k = 1; k < W; ++k) {
+                    const int o = (k << log_r) + warp;
+                    const float pm = ml_s[o][0];
+                    if (pm == -INFINITY) continue;
+                    const float mn = fmaxf(m, pm), f0 = m == -INFINITY ? 0.f : ex2_approx(m - mn), f1 = ex2_approx(pm - mn);
+                    const float4 v = acc_s[o][lane];
+                    m = mn;
+                    l = l * f0 + ml_s[o][1] * f1;
+                    a.x = a.x * f0 + v.x * f1;
+                    a.y = a.y * f0 + v.y * f1;
+                    a.z = a.z * f0 + v.z * f1;
+                    a.w = a.w * f0 + v.w * f1;
+                }
+        }
+        if (piece == 0 && r < rows) {
+            const float il = m == -INFINITY ? 0.f : 1.0f / l;
+            const int rr = tile * ROWS + r;
+            T* dst = reinterpret_cast<T*>(p.out) + (w.q0 + rr / G) * p.out_stride + (h * G + rr % G) * HD + 4 * lane;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f<T>(a.x * il, a.y * il), pack_f<T>(a.z * il, a.w * il));
+        }
     }
 }
 
