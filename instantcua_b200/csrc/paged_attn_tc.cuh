@@ -8,7 +8,7 @@
 //   O_t += P_t V      (A = P_t from tensor memory, B = V as it lies in the cache: MN-major)
 // warps 0-3 / 4-7  softmax of half 0 / 1, one thread per row (tensor-memory lane)
 // warp 8           tensor memory, and the one thread that issues every product
-// warps 9-12       bring the q rows and the K / V blocks: 16-bit rows by cp.async into the 128-byte
+// warps 12-15      bring the q rows and the K / V blocks: 16-bit rows by cp.async into the 128-byte
 //                  swizzle (which is the cache's own row order), q8 rows through registers, converted
 //                  exactly; rows past the sequence's end and of pages that do not exist are zeros
 // While one half's softmax runs, the tensor core works for the other half.  The running maximum is
@@ -26,7 +26,10 @@ namespace icua {
 
 constexpr int PC_BK = 128;
 constexpr int PC_ROWS = 256;
-constexpr int PC_THREADS = 13 * 32;
+constexpr int PC_THREADS = 16 * 32;
+// Registers per thread after the split of the launch's 512 x 128: softmax, products, producers.
+constexpr int PC_REGS_SOFTMAX = 184, PC_REGS_MMA = 56, PC_REGS_LOAD = 88;
+static_assert(2 * PC_REGS_SOFTMAX + PC_REGS_MMA + PC_REGS_LOAD <= 512, "the split draws on the launch's registers");
 constexpr int PC_TMEM_COLS = 512;  // S / P of the halves at 0, 128; O at 256, 384
 constexpr int PC_PART = PC_ROWS * HD + 2 * PC_ROWS;  // floats of a part: o[256][128], m[256], l[256]
 
@@ -65,22 +68,65 @@ __host__ __device__ constexpr uint32_t pc_idesc(bool b_mn) {
     return umma_idesc_f16(128, 128) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
 }
 
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// 32 columns from `taddr` into v[OFF ..]; complete after tmem_wait_ld.
+template <int OFF, int N>
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float (&v)[N]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=f"(v[OFF + 0]), "=f"(v[OFF + 1]), "=f"(v[OFF + 2]), "=f"(v[OFF + 3]), "=f"(v[OFF + 4]), "=f"(v[OFF + 5]),
+          "=f"(v[OFF + 6]), "=f"(v[OFF + 7]), "=f"(v[OFF + 8]), "=f"(v[OFF + 9]), "=f"(v[OFF + 10]), "=f"(v[OFF + 11]),
+          "=f"(v[OFF + 12]), "=f"(v[OFF + 13]), "=f"(v[OFF + 14]), "=f"(v[OFF + 15]), "=f"(v[OFF + 16]), "=f"(v[OFF + 17]),
+          "=f"(v[OFF + 18]), "=f"(v[OFF + 19]), "=f"(v[OFF + 20]), "=f"(v[OFF + 21]), "=f"(v[OFF + 22]), "=f"(v[OFF + 23]),
+          "=f"(v[OFF + 24]), "=f"(v[OFF + 25]), "=f"(v[OFF + 26]), "=f"(v[OFF + 27]), "=f"(v[OFF + 28]), "=f"(v[OFF + 29]),
+          "=f"(v[OFF + 30]), "=f"(v[OFF + 31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, float (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+          "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+// (the values pass through, so that no use of them moves above the wait)
+template <int N>
+__device__ __forceinline__ void tmem_wait_ld(float (&v)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
+}
+
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
-    uint32_t a[16], b[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        a[i] = __float_as_uint(v[i]);
-        b[i] = __float_as_uint(v[16 + i]);
-    }
-    tmem_st16(taddr, a);
-    tmem_st16(taddr + 16, b);
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -190,9 +236,10 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
         return last < 0 ? 0 : max(0, min(t.j1, last / PC_BK + 1) - t.j0);
     };
 
-    if (warp >= 9) {
+    if (warp >= 12) {
+        reg_dec<PC_REGS_LOAD>();
         // ---- producers -----------------------------------------------------------------------------
-        const int w = warp - 9;
+        const int w = warp - 12;
         bool ok = true;
         {
             const T* qrow[2];
@@ -334,9 +381,10 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
             }
         }
         if (!ok && lane == 0 && p.err) atomicOr(p.err, ERR_WAIT_PREFILL);
-    } else if (warp == 8) {
+    } else if (warp >= 8) {
+        reg_dec<PC_REGS_MMA>();
         // ---- products --------------------------------------------------------------------------------
-        if (lane == 0) {
+        if (warp == 8 && lane == 0) {
             const int nb[2] = {half_blocks(0), half_blocks(1)};
             const uint32_t id_s = pc_idesc<T>(false), id_o = pc_idesc<T>(true);
             bool ok = mbar_wait_bounded(q_full, 0);
@@ -384,13 +432,15 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
             mbar_wait_bounded(done, 0);
         }
     } else {
+        reg_inc<PC_REGS_SOFTMAX>();
         // ---- softmax ---------------------------------------------------------------------------------
         const int hf = warp >> 2, quarter = warp & 3;
         const int R = t.row0 + 128 * hf + 32 * quarter + lane;
         const int lim = R < rows ? t.kv - t.n + R / G : -1;
         const int nb = half_blocks(hf);
         const uint32_t s_tm = tmem + 128 * hf + ((uint32_t)(32 * quarter) << 16), o_tm = s_tm + 256;
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY;
+        float2 l = make_float2(0.f, 0.f);  // sums of the even and of the odd keys
         bool ok = true;
         for (int i = 0; i < nb; ++i) {
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(&s_full[hf], i & 1))) {
@@ -405,53 +455,71 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
                 ok = false;
                 break;
             }
-            // this row's score of key c of the block, in units of log2
-            auto score = [&](float s, int c) {
-                s = Q8 ? fmaf(s, f[c], f[128 + c]) : s * p.scale_log2;
-                return edge && k0 + c > lim ? -INFINITY : s;
-            };
-            float bm = -INFINITY;
+            float v[128];
+            tmem_ld32_async<0>(s_tm, v);
+            tmem_ld32_async<32>(s_tm + 32, v);
+            tmem_ld32_async<64>(s_tm + 64, v);
+            tmem_ld32_async<96>(s_tm + 96, v);
+            tmem_wait_ld(v);
+            if (Q8) {  // scores in units of log2, with the V scale's logarithm
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float v[64];
-                tmem_ld64(s_tm + 64 * c, v);
-#pragma unroll
-                for (int e = 0; e < 64; ++e) bm = fmaxf(bm, score(v[e], 64 * c + e));
+                for (int c = 0; c < 32; ++c) {
+                    const float4 a = reinterpret_cast<const float4*>(f)[c], b = reinterpret_cast<const float4*>(f + 128)[c];
+                    const float2 x = fma2(make_float2(v[4 * c], v[4 * c + 1]), make_float2(a.x, a.y), make_float2(b.x, b.y));
+                    const float2 y = fma2(make_float2(v[4 * c + 2], v[4 * c + 3]), make_float2(a.z, a.w), make_float2(b.z, b.w));
+                    v[4 * c] = x.x; v[4 * c + 1] = x.y; v[4 * c + 2] = y.x; v[4 * c + 3] = y.y;
+                }
             }
+            if (edge) {
+#pragma unroll
+                for (int c = 0; c < 128; ++c)
+                    if (k0 + c > lim) v[c] = -INFINITY;
+            }
+            float bm4[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                bm4[c] = fmaxf(v[c], v[c + 4]);
+#pragma unroll
+                for (int e = 8; e < 128; e += 8) bm4[c] = fmaxf(bm4[c], fmaxf(v[e + c], v[e + c + 4]));
+            }
+            const float sl = Q8 ? 1.f : p.scale_log2;
+            const float bm = fmaxf(fmaxf(bm4[0], bm4[1]), fmaxf(bm4[2], bm4[3])) * sl;
             const bool move = bm > m + 8.f;  // (from -inf: any finite score)
             if (__any_sync(0xffffffffu, move)) {
-                const float corr = move ? (m == -INFINITY ? 0.f : exp2f(m - bm)) : 1.f;
+                const float corr = move ? (m == -INFINITY ? 0.f : ex2_approx(m - bm)) : 1.f;
                 if (move) m = bm;
-                l *= corr;
+                l.x *= corr;
+                l.y *= corr;
                 if (i > 0) {  // (O is complete up to the block before: S of this one was issued after it)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float v[32];
-                        tmem_ld32(o_tm + 32 * c, v);
+                    for (int c = 0; c < 8; ++c) {
+                        float x[16];
+                        uint32_t r[16];
+                        tmem_ld16_async(o_tm + 16 * c, x);
+                        tmem_wait_ld(x);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) v[e] *= corr;
-                        tmem_st32(o_tm + 32 * c, v);
+                        for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(x[e] * corr);
+                        tmem_st16(o_tm + 16 * c, r);
                     }
                 }
             }
-            const float ms = m == -INFINITY ? 0.f : m;
+            const float ms = m == -INFINITY ? 0.f : -m;
+            const float2 sl2 = make_float2(sl, sl), ms2 = make_float2(ms, ms);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float v[64];
-                tmem_ld64(s_tm + 64 * c, v);
+            for (int c = 0; c < 4; ++c) {
+                uint32_t r[16];
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    uint32_t r[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int x = 64 * c + 32 * b + 2 * e;
-                        const float e0 = ex2_approx(score(v[32 * b + 2 * e], x) - ms);
-                        const float e1 = ex2_approx(score(v[32 * b + 2 * e + 1], x + 1) - ms);
-                        l += Q8 ? fmaf(e0, f[256 + x], e1 * f[257 + x]) : e0 + e1;
-                        r[e] = pack_f<T>(e0, e1);
-                    }
-                    tmem_st16(s_tm + 32 * c + 16 * b, r);
+                for (int e = 0; e < 16; ++e) {
+                    const int x = 32 * c + 2 * e;
+                    float2 z = make_float2(v[x], v[x + 1]);
+                    z = Q8 ? add2(z, ms2) : fma2(z, sl2, ms2);
+                    z.x = ex2_approx(z.x);
+                    z.y = ex2_approx(z.y);
+                    if (Q8) l = fma2(z, *reinterpret_cast<const float2*>(f + 256 + x), l);
+                    else l = add2(l, z);
+                    r[e] = pack_f<T>(z.x, z.y);
                 }
+                tmem_st16(s_tm + 16 * c, r);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -464,7 +532,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
             if (lane == 0 && p.err) atomicOr(p.err, ERR_WAIT_PREFILL);
         } else {
             const bool real = R < rows;
-            const float il = p.n_split > 1 ? 1.f : m == -INFINITY ? 0.f : 1.0f / l;
+            const float il = p.n_split > 1 ? 1.f : m == -INFINITY ? 0.f : 1.0f / (l.x + l.y);
             const int Rc = min(R, rows - 1);
             T* dst = reinterpret_cast<T*>(p.out) + (t.q0 + Rc / G) * p.out_stride + (h * G + Rc % G) * HD;
             float* pt = p.part + (size_t)blockIdx.x * PC_PART;
@@ -486,7 +554,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
             }
             if (p.n_split > 1) {
                 pt[PC_ROWS * HD + rt] = m;
-                pt[PC_ROWS * HD + PC_ROWS + rt] = l;
+                pt[PC_ROWS * HD + PC_ROWS + rt] = l.x + l.y;
             }
         }
     }
