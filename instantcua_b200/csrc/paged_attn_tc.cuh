@@ -4,7 +4,8 @@
 // x 128; one CTA takes a tile over all its keys, or over a share of them (n_split) when there are fewer
 // tiles than SMs.  Per block of 128 keys and half t:
 //   S_t = Q_t K^T     (M = 128, N = 128, K = 128; both operands K-major in shared memory)
-//   P_t = 2^(S_t scale log2(e) - m)   in the 16-bit type of q, written over S_t in tensor memory
+//   P_t = 2^(S_t scale log2(e) - m)   in the 16-bit type of q, written over S_t in tensor memory, 64 keys
+//                                     at a time so that the product with V starts early
 //   O_t += P_t V      (A = P_t from tensor memory, B = V as it lies in the cache: MN-major)
 // warps 0-3 / 4-7  softmax of half 0 / 1, one thread per row (tensor-memory lane)
 // warp 8           tensor memory, and the one thread that issues every product
@@ -39,7 +40,7 @@ struct PcSmem {
     static constexpr int v_off = k_off + 2 * 32768;
     static constexpr int c_off = v_off + 2 * 32768;       // q8: 4 x (mul, add, inv)[128]
     static constexpr int bar_off = c_off + 4 * 3 * 512;
-    static constexpr int total = bar_off + 20 * 8;
+    static constexpr int total = bar_off + 22 * 8;
     static constexpr int alloc = total + 1024;
 };
 
@@ -66,6 +67,17 @@ __device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t saddr, uint32_t 
 template <typename T>
 __host__ __device__ constexpr uint32_t pc_idesc(bool b_mn) {
     return umma_idesc_f16(128, 128) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
+}
+
+// Whether the phase has completed (try_wait would suspend the thread until it has, or for a while).
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 
 template <int N>
@@ -187,7 +199,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
     uint8_t* smem = smem_raw + (((base_u + 1023u) & ~1023u) - base_u);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::bar_off);
     uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7, *s_full = bars + 9,
-             *p_full = bars + 11, *o_full = bars + 13, *done = bars + 15, *c_full = bars + 16;
+             *p_full = bars + 11, *o_full = bars + 15, *done = bars + 17, *c_full = bars + 18;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n_kv = p.pages.n_kv, G = p.group, ps_shift = p.pages.ps_shift;
     const int h = blockIdx.x % n_kv, split = (blockIdx.x / n_kv) % p.n_split, y = blockIdx.x / (n_kv * p.n_split);
@@ -209,6 +221,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
             mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[2 + i], 4);
             mbar_init(&o_full[i], 1);
         }
         for (int i = 0; i < 4; ++i) mbar_init(&c_full[i], 128);
@@ -269,65 +282,88 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
             fence_proxy_async_smem();
             mbar_arrive(q_full);
         }
-        // pool row of key 32 w + lane of block j (all ones: none)
-        auto key_row = [&](int j) -> uint32_t {
-            const int pos = j * PC_BK + 32 * w + lane;
-            if (pos >= t.kv) return 0xffffffffu;
-            const long long r = page_row(p.pages, p.seqs, t.s, h, pos, p.err);
-            return r < 0 ? 0xffffffffu : (uint32_t)r;
+        // This warp's keys 32 w .. 32 w + 31 of a block lie in two pages at most, sixteen each.  The table is
+        // read one block ahead (raw entries; -2: past the sequence's end).
+        const int* table = p.seqs.table + (long long)t.s * p.seqs.max_pages;
+        auto entry = [&](int j, int part) -> int {
+            const int pos = j * PC_BK + 32 * w + 16 * part;
+            return j < t.j1 && pos < t.kv ? table[pos >> ps_shift] : -2;
         };
+        // pool row of the first of the sixteen keys (all ones: none of them is to be read)
+        auto row_of = [&](int page, int j, int part) -> uint32_t {
+            if ((unsigned)page >= (unsigned)p.pages.n_pages) {
+                if (page != -2 && lane == 0 && p.err) atomicOr(p.err, ERR_PAGE);
+                return 0xffffffffu;
+            }
+            const int pos = j * PC_BK + 32 * w + 16 * part;
+            return (uint32_t)(page * p.pages.page_rows + h * p.pages.head_rows + (pos & ((1 << ps_shift) - 1)));
+        };
+        int ahead[2] = {entry(t.j0, 0), entry(t.j0, 1)};
         if (!Q8) {
             const int c = lane & 15;
-            auto issue = [&](uint8_t* dst, const uint8_t* pool, uint32_t row) {
-                const uint32_t d = smem_u32(dst) + (c >> 3) * 16384 + (c & 7) * 16 + (32 * w) * 128;
+            // rows 2 k + lane / 16 of each sixteen; `left`: the sequence's keys from the first one on
+            auto issue = [&](uint8_t* dst, const uint8_t* pool, const uint32_t (&row)[2], int left) {
+                const uint32_t d = smem_u32(dst) + (c >> 3) * 16384 + (c & 7) * 16 + (32 * w + (lane >> 4)) * 128;
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const int src = 2 * k + (lane >> 4);
-                    const uint32_t r = __shfl_sync(0xffffffffu, row, src);
-                    const bool rl = r != 0xffffffffu;
-                    cp_async16(d + src * 128, pool + (rl ? (size_t)r * 256 + c * 16 : 0), rl);
+                for (int part = 0; part < 2; ++part) {
+                    const bool there = row[part] != 0xffffffffu;
+                    const uint8_t* src = pool + (there ? (size_t)row[part] * 256 : 0) + lane * 16;
+                    const int n = there ? left - 16 * part - (lane >> 4) : 0;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) cp_async16(d + part * 2048 + k * 256, src + (2 * k < n ? k * 512 : 0), 2 * k < n);
                 }
                 cp_async_commit();
             };
-            uint32_t row = nblk > 0 ? key_row(t.j0) : 0;
-            for (int i = 0; i < nblk; ++i) {
-                const int st = i & 1;
-                const uint32_t next = i + 1 < nblk ? key_row(t.j0 + i + 1) : 0;
-                if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait_bounded(&k_empty[st], ((i >> 1) - 1) & 1))) { ok = false; break; }
-                issue(smem + S::k_off + st * 32768, p.pages.k, row);
-                if (i >= 1) {  // two copies stay in flight: K of the block before has landed
-                    cp_async_wait<2>();
-                    fence_proxy_async_smem();
-                    mbar_arrive(&k_full[(i - 1) & 1]);
-                }
-                if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait_bounded(&v_empty[st], ((i >> 1) - 1) & 1))) { ok = false; break; }
-                issue(smem + S::v_off + st * 32768, p.pages.v, row);
-                if (i >= 1) {
-                    cp_async_wait<2>();
-                    fence_proxy_async_smem();
-                    mbar_arrive(&v_full[(i - 1) & 1]);
-                }
-                row = next;
-            }
-            if (ok && nblk > 0) {
-                cp_async_wait<1>();
+            // Copies are announced one item (the K or V of a block) behind, two in flight, so that their
+            // latency is covered; a producer that has to wait for room announces everything first.
+            int told = 0, sent = 0;  // items, K and V in turn
+            auto tell = [&]() {
                 fence_proxy_async_smem();
-                mbar_arrive(&k_full[(nblk - 1) & 1]);
-                cp_async_wait<0>();
-                fence_proxy_async_smem();
-                mbar_arrive(&v_full[(nblk - 1) & 1]);
+                mbar_arrive((told & 1 ? v_full : k_full) + ((told >> 1) & 1));
+                ++told;
+            };
+            for (int i = 0; ok && i < nblk; ++i) {
+                const int st = i & 1, j = t.j0 + i;
+                const uint32_t row[2] = {row_of(ahead[0], j, 0), row_of(ahead[1], j, 1)};
+                ahead[0] = entry(j + 1, 0);
+                ahead[1] = entry(j + 1, 1);
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    if (i >= 2) {
+                        uint64_t* room = (kv ? v_empty : k_empty) + st;
+                        const uint32_t ph = ((i >> 1) - 1) & 1;
+                        if (!__all_sync(0xffffffffu, mbar_test(room, ph))) {
+                            cp_async_wait<0>();
+                            while (told < sent) tell();
+                            if (!__all_sync(0xffffffffu, mbar_wait_bounded(room, ph))) {
+                                ok = false;
+                                break;
+                            }
+                        }
+                    }
+                    issue(smem + (kv ? S::v_off : S::k_off) + st * 32768, kv ? p.pages.v : p.pages.k, row, t.kv - j * PC_BK - 32 * w);
+                    ++sent;
+                    cp_async_wait<2>();
+                    while (told < sent - 2) tell();
+                }
             }
             cp_async_wait<0>();
+            while (told < sent) tell();
         } else {
             // eight 16-byte loads a lane: rows 4 i + lane / 8 of the warp's 32, chunk lane % 8
             const int c = lane & 7;
             uint4 rk[8], rv[8];
-            auto load = [&](uint4 (&raw)[8], const uint8_t* pool, uint32_t row) {
+            auto load = [&](uint4 (&raw)[8], const uint8_t* pool, const uint32_t (&row)[2], int left) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t r = __shfl_sync(0xffffffffu, row, 4 * i + (lane >> 3));
-                    raw[i] = make_uint4(0, 0, 0, 0);
-                    if (r != 0xffffffffu) raw[i] = *reinterpret_cast<const uint4*>(pool + (size_t)r * HD + c * 16);
+                for (int part = 0; part < 2; ++part) {
+                    const bool there = row[part] != 0xffffffffu;
+                    const uint8_t* src = pool + (there ? (size_t)row[part] * HD : 0) + lane * 16;
+                    const int n = there ? left - 16 * part - (lane >> 3) : 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        raw[4 * part + i] = make_uint4(0, 0, 0, 0);
+                        if (4 * i < n) raw[4 * part + i] = *reinterpret_cast<const uint4*>(src + i * 512);
+                    }
                 }
             };
             // 16 codes become two chunks of the 128-byte swizzle; the two halves of the row in turn, so that
@@ -351,14 +387,16 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
                     *reinterpret_cast<uint4*>(d + (((p0 + !odd) ^ (R & 7)) << 4)) = odd ? lo : hi;
                 }
             };
-            uint32_t row = nblk > 0 ? key_row(t.j0) : 0xffffffffu;
-            load(rk, p.pages.k, row);
+            uint32_t row[2] = {row_of(ahead[0], t.j0, 0), row_of(ahead[1], t.j0, 1)};
+            if (nblk > 0) load(rk, p.pages.k, row, t.kv - t.j0 * PC_BK - 32 * w);
             for (int i = 0; i < nblk; ++i) {
-                const int st = i & 1;
-                load(rv, p.pages.v, row);
-                const bool rl = row != 0xffffffffu;
-                const float ksc = rl ? p.pages.ks[row] : 0.f, vsc = rl ? p.pages.vs[row] : 1.f;
-                const uint32_t next = i + 1 < nblk ? key_row(t.j0 + i + 1) : 0xffffffffu;
+                const int st = i & 1, j = t.j0 + i, left = t.kv - j * PC_BK - 32 * w;
+                ahead[0] = entry(j + 1, 0);
+                ahead[1] = entry(j + 1, 1);
+                load(rv, p.pages.v, row, left);
+                const uint32_t mine = row[lane >> 4];
+                const bool rl = mine != 0xffffffffu && lane < left;
+                const float ksc = rl ? p.pages.ks[mine + (lane & 15)] : 0.f, vsc = rl ? p.pages.vs[mine + (lane & 15)] : 1.f;
                 if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait_bounded(&k_empty[st], ((i >> 1) - 1) & 1))) { ok = false; break; }
                 store(smem + S::k_off + st * 32768, rk);
                 {
@@ -372,12 +410,13 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
                 }
                 fence_proxy_async_smem();
                 mbar_arrive(&k_full[st]);
-                load(rk, p.pages.k, next);
+                row[0] = row_of(ahead[0], j + 1, 0);
+                row[1] = row_of(ahead[1], j + 1, 1);
+                if (i + 1 < nblk) load(rk, p.pages.k, row, left - PC_BK);
                 if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait_bounded(&v_empty[st], ((i >> 1) - 1) & 1))) { ok = false; break; }
                 store(smem + S::v_off + st * 32768, rv);
                 fence_proxy_async_smem();
                 mbar_arrive(&v_full[st]);
-                row = next;
             }
         }
         if (!ok && lane == 0 && p.err) atomicOr(p.err, ERR_WAIT_PREFILL);
@@ -389,6 +428,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
             const uint32_t id_s = pc_idesc<T>(false), id_o = pc_idesc<T>(true);
             bool ok = mbar_wait_bounded(q_full, 0);
             tc_fence_after();
+            auto last_half = [&](int i) { return i < nb[1] ? 1 : 0; };
             auto scores = [&](int hf, int i) {
                 const uint64_t qd = umma_desc_sw128(smem_u32(smem + S::q_off + hf * 32768));
                 const uint64_t kd = umma_desc_sw128(smem_u32(smem + S::k_off + (i & 1) * 32768));
@@ -414,17 +454,21 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
                 if (i + 1 < nblk && !(ok = mbar_wait_bounded(&k_full[(i + 1) & 1], ((i + 1) >> 1) & 1))) break;
                 for (int hf = 0; ok && hf < 2; ++hf) {
                     if (i >= nb[hf]) continue;
-                    if (!(ok = mbar_wait_bounded(&p_full[hf], i & 1))) break;
-                    tc_fence_after();
                     const uint64_t vd = umma_desc_sw128_mn(smem_u32(smem + S::v_off + st * 32768), 16384);
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks)
-                        tc_mma_f16_ts(tmem + 256 + 128 * hf, tmem + 128 * hf + 8 * ks, vd + 128 * ks, id_o, (i | ks) != 0);
+                    for (int part = 0; part < 2; ++part) {  // the keys' first half as soon as its P is there
+                        if (!(ok = mbar_wait_bounded(&p_full[2 * part + hf], i & 1))) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int ks = 4 * part; ks < 4 * part + 4; ++ks)
+                            tc_mma_f16_ts(tmem + 256 + 128 * hf, tmem + 128 * hf + 8 * ks, vd + 128 * ks, id_o, (i | ks) != 0);
+                    }
+                    if (!ok) break;
+                    if (hf == last_half(i)) tc_commit(&v_empty[st]);
                     if (i + 1 < nb[hf]) scores(hf, i + 1);
                     else tc_commit(&o_full[hf]);
                 }
                 if (!ok) break;
-                tc_commit(&v_empty[st]);
                 if (i + 1 < nblk) tc_commit(&k_empty[(i + 1) & 1]);
             }
             if (!ok && p.err) atomicOr(p.err, ERR_WAIT_PREFILL);
@@ -520,11 +564,13 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
                     r[e] = pack_f<T>(z.x, z.y);
                 }
                 tmem_st16(s_tm + 16 * c, r);
+                if (c & 1) {
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[(c & 2) + hf]);
+                }
             }
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[hf]);
         }
         if (ok && nb > 0 && !__all_sync(0xffffffffu, mbar_wait_bounded(&o_full[hf], 0))) ok = false;
         tc_fence_after();
