@@ -201,9 +201,9 @@ TcGrid tc_grid(const icua_kv_seqs* s, int n_kv, int group, int min_rows, int n_s
 
 template <typename T, bool Q8>
 cudaError_t launch_attn_tc(const PagedTcParams& p, int tiles, int dev, cudaStream_t st) {
-    cudaError_t e = allow_smem<paged_attn_tc_kernel<T, Q8>>(PcSmem::alloc, dev);
+    cudaError_t e = allow_smem<paged_attn_tc_kernel<T, Q8>>(PcSmem<Q8>::alloc, dev);
     if (e != cudaSuccess) return e;
-    paged_attn_tc_kernel<T, Q8><<<tiles * p.pages.n_kv * p.n_split, PC_THREADS, PcSmem::alloc, st>>>(p);
+    paged_attn_tc_kernel<T, Q8><<<tiles * p.pages.n_kv * p.n_split, PC_THREADS, PcSmem<Q8>::alloc, st>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess || p.n_split == 1) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles * p.pages.n_kv * 32);

@@ -34,14 +34,30 @@ static_assert(2 * PC_REGS_SOFTMAX + PC_REGS_MMA + PC_REGS_LOAD <= 512, "the spli
 constexpr int PC_TMEM_COLS = 512;  // S / P of the halves at 0, 128; O at 256, 384
 constexpr int PC_PART = PC_ROWS * HD + 2 * PC_ROWS;  // floats of a part: o[256][128], m[256], l[256]
 
+// K and V blocks in turn (item 2 i: K of block i, 2 i + 1: V) through one ring of tiles.
+template <bool Q8>
 struct PcSmem {
+    static constexpr int NS = Q8 ? 4 : 5;
     static constexpr int q_off = 0;                       // 2 halves x [2][128 rows][128 B]
-    static constexpr int k_off = 65536;                   // 2 stages x [2][128 keys][128 B]
-    static constexpr int v_off = k_off + 2 * 32768;
-    static constexpr int c_off = v_off + 2 * 32768;       // q8: 4 x (mul, add, inv)[128]
-    static constexpr int bar_off = c_off + 4 * 3 * 512;
-    static constexpr int total = bar_off + 22 * 8;
+    static constexpr int kv_off = 65536;                  // NS x [2][128 keys][128 B]
+    static constexpr int c_off = kv_off + NS * 32768;     // q8: 4 x (mul, add, inv)[128]
+    static constexpr int bar_off = c_off + (Q8 ? 4 * 3 * 512 : 0);
+    static constexpr int total = bar_off + 24 * 8;
     static constexpr int alloc = total + 1024;
+};
+// Place of an item in the ring.
+template <int NS>
+struct PcRing {
+    int slot = 0;
+    uint32_t lap = 0;
+    __device__ __forceinline__ void next() {
+        if (++slot == NS) {
+            slot = 0;
+            ++lap;
+        }
+    }
+    __device__ __forceinline__ uint32_t full_phase() const { return lap & 1; }
+    __device__ __forceinline__ uint32_t empty_phase() const { return (lap - 1) & 1; }  // laps after the first
 };
 
 struct PagedTcParams {
@@ -58,15 +74,34 @@ struct PagedTcParams {
     int* err;
 };
 
-// Shared-memory descriptor of an MN-major operand in the 128-byte swizzle: 64-element groups of the M / N
-// index `lbo` bytes apart, groups of eight K rows 1,024 bytes apart.
-__device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t saddr, uint32_t lbo) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
 template <typename T>
 __host__ __device__ constexpr uint32_t pc_idesc(bool b_mn) {
     return umma_idesc_f16(128, 128) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u);
+}
+
+// Products of the 128-byte swizzle with the descriptors' changing words alone in registers (the upper one
+// is the same for all K-major operands, and one other for V).  Issued by the lane that `one` marks, from a
+// warp that stays together: the operands then live in uniform registers and an issue costs little more
+// than the instruction itself.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
+constexpr uint32_t PC_DESC_HI = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void pc_mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate, uint32_t one) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 a, {%1, %3};\n\t"
+        "mov.b64 b, {%2, %3};\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+        "r"(a_lo), "r"(b_lo), "n"(PC_DESC_HI), "r"(idesc), "r"(accumulate), "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ void pc_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate, uint32_t one) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b_lo), "n"(PC_DESC_HI), "r"(idesc), "r"(accumulate), "r"(one)
+        : "memory");
 }
 
 // Whether the phase has completed (try_wait would suspend the thread until it has, or for a while).
@@ -190,7 +225,8 @@ __device__ __forceinline__ void pc_share(PcTile& t, int G, int split, int n_spli
 // Grid: n_kv x n_split x (a bound of the) tiles, kv head fastest.
 template <typename T, bool Q8>
 __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const PagedTcParams p) {
-    using S = PcSmem;
+    using S = PcSmem<Q8>;
+    constexpr int NS = S::NS;
     extern __shared__ uint8_t smem_raw[];
     __shared__ PcTile tile_s;
     __shared__ int live_s;
@@ -198,8 +234,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
     const uint32_t base_u = smem_u32(smem_raw);
     uint8_t* smem = smem_raw + (((base_u + 1023u) & ~1023u) - base_u);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::bar_off);
-    uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7, *s_full = bars + 9,
-             *p_full = bars + 11, *o_full = bars + 15, *done = bars + 17, *c_full = bars + 18;
+    uint64_t *q_full = bars, *done = bars + 1, *s_full = bars + 2, *p_full = bars + 4, *o_full = bars + 8, *c_full = bars + 10,
+             *kv_full = bars + 14, *kv_empty = bars + 14 + NS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n_kv = p.pages.n_kv, G = p.group, ps_shift = p.pages.ps_shift;
     const int h = blockIdx.x % n_kv, split = (blockIdx.x / n_kv) % p.n_split, y = blockIdx.x / (n_kv * p.n_split);
@@ -215,16 +251,16 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
     } else if (threadIdx.x == 32) {
         mbar_init(q_full, 128);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&k_full[i], 128);
-            mbar_init(&k_empty[i], 1);
-            mbar_init(&v_full[i], 128);
-            mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
             mbar_init(&p_full[2 + i], 4);
             mbar_init(&o_full[i], 1);
         }
         for (int i = 0; i < 4; ++i) mbar_init(&c_full[i], 128);
+        for (int i = 0; i < NS; ++i) {
+            mbar_init(&kv_full[i], 128);
+            mbar_init(&kv_empty[i], 1);
+        }
         mbar_init(done, 1);
         fence_mbar_init();
     }
@@ -314,41 +350,40 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
                 }
                 cp_async_commit();
             };
-            // Copies are announced one item (the K or V of a block) behind, two in flight, so that their
-            // latency is covered; a producer that has to wait for room announces everything first.
-            int told = 0, sent = 0;  // items, K and V in turn
-            auto tell = [&]() {
+            // Copies are announced two items behind, three in flight, so that their latency is covered; a
+            // producer that has to wait for room announces everything first.
+            PcRing<NS> put, tell;
+            int untold = 0;
+            auto tell_one = [&]() {
                 fence_proxy_async_smem();
-                mbar_arrive((told & 1 ? v_full : k_full) + ((told >> 1) & 1));
-                ++told;
+                mbar_arrive(&kv_full[tell.slot]);
+                tell.next();
+                --untold;
             };
             for (int i = 0; ok && i < nblk; ++i) {
-                const int st = i & 1, j = t.j0 + i;
+                const int j = t.j0 + i;
                 const uint32_t row[2] = {row_of(ahead[0], j, 0), row_of(ahead[1], j, 1)};
                 ahead[0] = entry(j + 1, 0);
                 ahead[1] = entry(j + 1, 1);
 #pragma unroll
                 for (int kv = 0; kv < 2; ++kv) {
-                    if (i >= 2) {
-                        uint64_t* room = (kv ? v_empty : k_empty) + st;
-                        const uint32_t ph = ((i >> 1) - 1) & 1;
-                        if (!__all_sync(0xffffffffu, mbar_test(room, ph))) {
-                            cp_async_wait<0>();
-                            while (told < sent) tell();
-                            if (!__all_sync(0xffffffffu, mbar_wait_bounded(room, ph))) {
-                                ok = false;
-                                break;
-                            }
+                    if (put.lap > 0 && !__all_sync(0xffffffffu, mbar_test(&kv_empty[put.slot], put.empty_phase()))) {
+                        cp_async_wait<0>();
+                        while (untold > 0) tell_one();
+                        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&kv_empty[put.slot], put.empty_phase()))) {
+                            ok = false;
+                            break;
                         }
                     }
-                    issue(smem + (kv ? S::v_off : S::k_off) + st * 32768, kv ? p.pages.v : p.pages.k, row, t.kv - j * PC_BK - 32 * w);
-                    ++sent;
+                    issue(smem + S::kv_off + put.slot * 32768, kv ? p.pages.v : p.pages.k, row, t.kv - j * PC_BK - 32 * w);
+                    put.next();
+                    ++untold;
                     cp_async_wait<2>();
-                    while (told < sent - 2) tell();
+                    while (untold > 2) tell_one();
                 }
             }
             cp_async_wait<0>();
-            while (told < sent) tell();
+            while (untold > 0) tell_one();
         } else {
             // eight 16-byte loads a lane: rows 4 i + lane / 8 of the warp's 32, chunk lane % 8
             const int c = lane & 7;
@@ -387,18 +422,22 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
                     *reinterpret_cast<uint4*>(d + (((p0 + !odd) ^ (R & 7)) << 4)) = odd ? lo : hi;
                 }
             };
+            PcRing<NS> put;
+            auto room = [&]() {
+                return put.lap == 0 || __all_sync(0xffffffffu, mbar_wait_bounded(&kv_empty[put.slot], put.empty_phase()));
+            };
             uint32_t row[2] = {row_of(ahead[0], t.j0, 0), row_of(ahead[1], t.j0, 1)};
             if (nblk > 0) load(rk, p.pages.k, row, t.kv - t.j0 * PC_BK - 32 * w);
             for (int i = 0; i < nblk; ++i) {
-                const int st = i & 1, j = t.j0 + i, left = t.kv - j * PC_BK - 32 * w;
+                const int j = t.j0 + i, left = t.kv - j * PC_BK - 32 * w;
                 ahead[0] = entry(j + 1, 0);
                 ahead[1] = entry(j + 1, 1);
                 load(rv, p.pages.v, row, left);
                 const uint32_t mine = row[lane >> 4];
                 const bool rl = mine != 0xffffffffu && lane < left;
                 const float ksc = rl ? p.pages.ks[mine + (lane & 15)] : 0.f, vsc = rl ? p.pages.vs[mine + (lane & 15)] : 1.f;
-                if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait_bounded(&k_empty[st], ((i >> 1) - 1) & 1))) { ok = false; break; }
-                store(smem + S::k_off + st * 32768, rk);
+                if (!(ok = room())) break;
+                store(smem + S::kv_off + put.slot * 32768, rk);
                 {
                     // (block i + 4 is stored after the scores of block i + 2, which come after both halves' softmax of i)
                     float* f = reinterpret_cast<float*>(smem + S::c_off) + (i & 3) * 384 + 32 * w + lane;
@@ -409,70 +448,90 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
                     mbar_arrive(&c_full[i & 3]);
                 }
                 fence_proxy_async_smem();
-                mbar_arrive(&k_full[st]);
+                mbar_arrive(&kv_full[put.slot]);
+                put.next();
                 row[0] = row_of(ahead[0], j + 1, 0);
                 row[1] = row_of(ahead[1], j + 1, 1);
                 if (i + 1 < nblk) load(rk, p.pages.k, row, left - PC_BK);
-                if (i >= 2 && !__all_sync(0xffffffffu, mbar_wait_bounded(&v_empty[st], ((i >> 1) - 1) & 1))) { ok = false; break; }
-                store(smem + S::v_off + st * 32768, rv);
+                if (!(ok = room())) break;
+                store(smem + S::kv_off + put.slot * 32768, rv);
                 fence_proxy_async_smem();
-                mbar_arrive(&v_full[st]);
+                mbar_arrive(&kv_full[put.slot]);
+                put.next();
             }
         }
         if (!ok && lane == 0 && p.err) atomicOr(p.err, ERR_WAIT_PREFILL);
     } else if (warp >= 8) {
         reg_dec<PC_REGS_MMA>();
         // ---- products --------------------------------------------------------------------------------
-        if (warp == 8 && lane == 0) {
+        if (warp == 8) {
             const int nb[2] = {half_blocks(0), half_blocks(1)};
-            const uint32_t id_s = pc_idesc<T>(false), id_o = pc_idesc<T>(true);
-            bool ok = mbar_wait_bounded(q_full, 0);
+            const uint32_t one = elect_one(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint32_t q_lo = ((base_u + 1023u) & ~1023u) >> 4, kv_lo = q_lo + (S::kv_off >> 4);
+            constexpr uint32_t id_s = pc_idesc<T>(false), id_o = pc_idesc<T>(true);
+            auto wait = [&](uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait_bounded(bar, phase)); };
+            auto commit = [&](uint64_t* bar) {
+                if (one) tc_commit(bar);
+                __syncwarp();
+            };
+            bool ok = wait(q_full, 0);
             tc_fence_after();
-            auto last_half = [&](int i) { return i < nb[1] ? 1 : 0; };
-            auto scores = [&](int hf, int i) {
-                const uint64_t qd = umma_desc_sw128(smem_u32(smem + S::q_off + hf * 32768));
-                const uint64_t kd = umma_desc_sw128(smem_u32(smem + S::k_off + (i & 1) * 32768));
+            PcRing<NS> get;  // the next item to wait for
+            auto arrived = [&]() {
+                if (!wait(&kv_full[get.slot], get.full_phase())) return false;
+                get.next();
+                return true;
+            };
+            // (a leading byte offset of 16 bytes is ignored for K-major operands; V's 64-column halves are 16 KB apart)
+            auto scores = [&](int hf, int k_slot) {
+                const uint32_t a = q_lo + (1u << 16) + hf * 2048, b = kv_lo + (1u << 16) + k_slot * 2048;
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks) {
                     const int off = (ks >> 2) * 1024 + 2 * (ks & 3);
-                    tc_mma_f16(tmem + 128 * hf, qd + off, kd + off, id_s, ks != 0);
+                    pc_mma_ss(tm + 128 * hf, a + off, b + off, id_s, ks != 0, one);
                 }
-                tc_commit(&s_full[hf]);
+                commit(&s_full[hf]);
             };
             if (ok && nblk > 0) {
-                ok = mbar_wait_bounded(&k_full[0], 0);
+                ok = arrived();
                 tc_fence_after();
                 if (ok) {
                     for (int hf = 0; hf < 2; ++hf)
                         if (nb[hf] > 0) scores(hf, 0);
-                    tc_commit(&k_empty[0]);
+                    commit(&kv_empty[0]);
                 }
             }
             for (int i = 0; ok && i < nblk; ++i) {
-                const int st = i & 1;
-                if (!(ok = mbar_wait_bounded(&v_full[st], (i >> 1) & 1))) break;
-                if (i + 1 < nblk && !(ok = mbar_wait_bounded(&k_full[(i + 1) & 1], ((i + 1) >> 1) & 1))) break;
-                for (int hf = 0; ok && hf < 2; ++hf) {
-                    if (i >= nb[hf]) continue;
-                    const uint64_t vd = umma_desc_sw128_mn(smem_u32(smem + S::v_off + st * 32768), 16384);
+                const int v_slot = get.slot;
+                if (!(ok = arrived())) break;
+                const int k_slot = get.slot;
+                const uint32_t v_lo = kv_lo + ((16384u >> 4) << 16) + v_slot * 2048;
+                bool k_here = false;
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    if (!ok || i >= nb[hf]) continue;
 #pragma unroll
                     for (int part = 0; part < 2; ++part) {  // the keys' first half as soon as its P is there
-                        if (!(ok = mbar_wait_bounded(&p_full[2 * part + hf], i & 1))) break;
+                        if (!ok || !(ok = wait(&p_full[2 * part + hf], i & 1))) break;
                         tc_fence_after();
 #pragma unroll
                         for (int ks = 4 * part; ks < 4 * part + 4; ++ks)
-                            tc_mma_f16_ts(tmem + 256 + 128 * hf, tmem + 128 * hf + 8 * ks, vd + 128 * ks, id_o, (i | ks) != 0);
+                            pc_mma_ts(tm + 256 + 128 * hf, tm + 128 * hf + 8 * ks, v_lo + 128 * ks, id_o, ks == 0 ? i : 1, one);
                     }
                     if (!ok) break;
-                    if (hf == last_half(i)) tc_commit(&v_empty[st]);
-                    if (i + 1 < nb[hf]) scores(hf, i + 1);
-                    else tc_commit(&o_full[hf]);
+                    if (hf == (i < nb[1] ? 1 : 0)) commit(&kv_empty[v_slot]);
+                    if (i + 1 < nb[hf]) {
+                        if (!k_here && !(ok = arrived())) break;
+                        k_here = true;
+                        scores(hf, k_slot);
+                    } else {
+                        commit(&o_full[hf]);
+                    }
                 }
-                if (!ok) break;
-                if (i + 1 < nblk) tc_commit(&k_empty[(i + 1) & 1]);
+                if (ok && i + 1 < nblk) commit(&kv_empty[k_slot]);
             }
-            if (!ok && p.err) atomicOr(p.err, ERR_WAIT_PREFILL);
-            tc_commit(done);  // every product issued has completed before tensor memory is freed
+            if (!ok && one && p.err) atomicOr(p.err, ERR_WAIT_PREFILL);
+            commit(done);  // every product issued has completed before tensor memory is freed
             mbar_wait_bounded(done, 0);
         }
     } else {
