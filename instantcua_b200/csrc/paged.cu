@@ -155,11 +155,11 @@ bool q_type_fits(int dtype, int kvd) {
 
 template <typename T, bool Q8, int MT>
 cudaError_t launch_attn(const PagedAttnParams& p, int dev, cudaStream_t st) {
-    const int smem = pa_smem(Q8, MT);
-    cudaError_t e = allow_smem<paged_attn_kernel<T, Q8, MT>>(smem, dev);
+    const int smem = pa_smem(Q8, MT, 1);
+    cudaError_t e = allow_smem<paged_attn_kernel<T, Q8, MT, 1>>(smem, dev);
     if (e != cudaSuccess) return e;
     const int ctas = std::min(PA_MAX_CTAS, 2 * sm_count(dev));
-    paged_attn_kernel<T, Q8, MT><<<ctas, PA_THREADS, smem, st>>>(p);
+    paged_attn_kernel<T, Q8, MT, 1><<<ctas, PA_THREADS, smem, st>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
@@ -173,8 +173,34 @@ cudaError_t launch_attn(const PagedAttnParams& p, int dev, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<T, 16 * MT, pa_block(Q8)>, p, ctas);
 }
 
+// One cluster per (sequence, kv head), one launch.
+template <typename T, bool Q8>
+cudaError_t launch_attn_cluster(const PagedAttnParams& p, int dev, cudaStream_t st) {
+    const int smem = pa_smem(Q8, 1, PA_CLUSTER);
+    const cudaError_t e = allow_smem<paged_attn_kernel<T, Q8, 1, PA_CLUSTER>>(smem, dev);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.seqs.n_seqs * p.pages.n_kv * PA_CLUSTER);
+    cfg.blockDim = dim3(PA_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = PA_CLUSTER;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, paged_attn_kernel<T, Q8, 1, PA_CLUSTER>, p);
+}
+
 template <int MT>
-cudaError_t launch_attn_rows(const PagedAttnParams& p, bool f16, bool q8, int dev, cudaStream_t st) {
+cudaError_t launch_attn_rows(const PagedAttnParams& p, bool f16, bool q8, bool cluster, int dev, cudaStream_t st) {
+    if constexpr (MT == 1)
+        if (cluster)
+            return q8    ? (f16 ? launch_attn_cluster<__half, true>(p, dev, st) : launch_attn_cluster<__nv_bfloat16, true>(p, dev, st))
+                   : f16 ? launch_attn_cluster<__half, false>(p, dev, st)
+                         : launch_attn_cluster<__nv_bfloat16, false>(p, dev, st);
     return q8    ? (f16 ? launch_attn<__half, true, MT>(p, dev, st) : launch_attn<__nv_bfloat16, true, MT>(p, dev, st))
            : f16 ? launch_attn<__half, false, MT>(p, dev, st)
                  : launch_attn<__nv_bfloat16, false, MT>(p, dev, st);
@@ -183,6 +209,7 @@ cudaError_t launch_attn_rows(const PagedAttnParams& p, bool f16, bool q8, int de
 // Sequences with up to PA_ROWS_FEW query rows per kv head go through the warp-MMA kernel, more rows
 // through the tensor-core kernel.
 constexpr int PA_ROWS_FEW = 64;
+constexpr int PA_CLUSTER_KEYS = 4096;
 
 // Tiles of the tensor-core kernel: a bound from what the host knows, and the shares of the keys that fill
 // the SMs when the tiles alone do not (two blocks of keys per share at least).
@@ -362,7 +389,15 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
     }
     p.alone = !tc;
     if (e == cudaSuccess && !all_tc)
-        e = (int64_t)seqs->max_q * p.group > 16 ? launch_attn_rows<2>(p, f16, q8, dev, s) : launch_attn_rows<1>(p, f16, q8, dev, s);
+    {
+        const bool one_tile = (int64_t)seqs->max_q * p.group <= 16;
+        // Few items, up to PA_CLUSTER_KEYS keys each: a cluster per item does without the second launch.  Longer
+        // ones want every SM, and more of them fill the GPU by themselves.
+        const bool cluster = one_tile && seqs->max_kv <= PA_CLUSTER_KEYS &&
+                             (int64_t)seqs->n_seqs * pages->n_kv * PA_CLUSTER <= 2 * sm_count(dev);
+        if (cluster) p.max_rows = 16;
+        e = one_tile ? launch_attn_rows<1>(p, f16, q8, cluster, dev, s) : launch_attn_rows<2>(p, f16, q8, false, dev, s);
+    }
     return e == cudaSuccess ? ICUA_OK : cuda_fail("icua_attn_paged", e);
 }
 

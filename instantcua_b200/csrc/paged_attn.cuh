@@ -32,6 +32,8 @@ constexpr int PA_ROWS_MAX = 32;   // query rows per item: 16 or 32
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = PA_WARPS * 32;
 constexpr int PA_NS = 3;          // ring slots per warp
+constexpr int PA_ITEM = 2;
+constexpr int PA_CLUSTER = 8;     // CTAs that share an item in the small-batch form
 constexpr int PA_MAX_CTAS = 320;  // workspace slots are laid out for so many
 constexpr int PA_MAX_SEQS = 1024;
 constexpr int PA_PART = PA_ROWS_MAX * HD + 2 * PA_ROWS_MAX;  // floats of a part: o[32][128], m[32], l[32]
@@ -53,8 +55,21 @@ struct PagedAttnParams {
 constexpr int pa_keys(bool q8) { return q8 ? 32 : 16; }  // rows of a warp's slot
 constexpr int pa_block(bool q8) { return PA_WARPS * pa_keys(q8); }
 constexpr int pa_slot(bool q8) { return q8 ? 32 * 2 * HD + 2 * 32 * 4 : 16 * 2 * HD * 2; }
-constexpr int pa_smem(bool q8, int mt) {
-    return PA_WARPS * PA_NS * pa_slot(q8) + (mt > 1 ? mt * 16 * 2 * HD : 0) + (PA_MAX_SEQS + 1) * 4;
+constexpr int pa_smem(bool q8, int mt, int cl) {
+    return PA_WARPS * PA_NS * pa_slot(q8) + (mt > 1 ? mt * 16 * 2 * HD : 0) + (cl > 1 ? 0 : (PA_MAX_SEQS + 1) * 4);
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The float that CTA `rank` of the cluster has where `here` is in this one.
+__device__ __forceinline__ float ld_cluster(const float* here, uint32_t rank) {
+    const uint32_t a = smem_u32(here);
+    uint32_t ra;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(ra) : "r"(a), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ra));
+    return v;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
@@ -101,9 +116,12 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
     return r;
 }
 
-// The line of blocks: sequence s holds items(s) x nb(s) of them, item = kv head x tiles + tile.
+// The line of work: sequence s holds items(s) (item = kv head x tiles + tile) of PA_ITEM + nb(s) units, the
+// first PA_ITEM for beginning and ending an item, then one per block of keys.  (Without them the CTAs that get
+// the short sequences of a ragged batch have several times the others' work.)
 struct PaWork {
     int n, kv, q0, tiles, nb, items;
+    __device__ __forceinline__ int units() const { return nb + PA_ITEM; }
 };
 __device__ __forceinline__ PaWork pa_work(const SeqsView& S, int ps_shift, int n_kv, int group, int max_rows, int tile_rows,
                                           int block, int s, int* err, bool alone = false) {
@@ -120,7 +138,7 @@ __device__ __forceinline__ PaWork pa_work(const SeqsView& S, int ps_shift, int n
     return w;
 }
 
-// pre[s] = blocks before sequence s, pre[n_seqs] = all of them.  `warp_tot` holds one word per warp.
+// pre[s] = units before sequence s, pre[n_seqs] = all of them.  `warp_tot` holds one word per warp.
 template <int THREADS>
 __device__ __forceinline__ uint32_t pa_prefix(const SeqsView& S, int ps_shift, int n_kv, int group, int max_rows, int tile_rows,
                                               int block, uint32_t* pre, uint32_t* warp_tot, int* err, bool alone = false) {
@@ -131,7 +149,7 @@ __device__ __forceinline__ uint32_t pa_prefix(const SeqsView& S, int ps_shift, i
         uint32_t w = 0;
         if (s < S.n_seqs) {
             const PaWork k = pa_work(S, ps_shift, n_kv, group, max_rows, tile_rows, block, s, err, alone);
-            w = (uint32_t)k.items * (uint32_t)k.nb;
+            w = (uint32_t)k.items * (uint32_t)k.units();
         }
         uint32_t x = w;
 #pragma unroll
@@ -179,63 +197,99 @@ struct PaDeal {
 };
 
 // MT: tiles of sixteen query rows per item that share every K and V fragment.
-template <typename T, bool Q8, int MT>
+// CL > 1 (few sequences of moderate length): no line; the cluster's CL CTAs share one item, (sequence, kv
+// head) of the cluster's number, and join its parts through distributed shared memory.  One launch and no
+// workspace, for calls whose time is latency.
+template <typename T, bool Q8, int MT, int CL>
 __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAttnParams p) {
     constexpr int KEYS = pa_keys(Q8), BLOCK = pa_block(Q8), SLOT = pa_slot(Q8), NT = KEYS / 8, ROWS = 16 * MT;
     constexpr int ROW = Q8 ? HD : 2 * HD;  // bytes of a cached row
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ float ml[PA_WARPS][2][ROWS];
+    __shared__ float ml_c[2][ROWS];  // CL > 1: this CTA's part's
     __shared__ uint32_t warp_tot[PA_WARPS];
     uint8_t* q_tile = smem + PA_WARPS * PA_NS * SLOT;  // MT > 1: the rows of the item, 256 B each, chunk c at c ^ (row & 7)
     uint32_t* pre = reinterpret_cast<uint32_t*>(q_tile + (MT > 1 ? ROWS * 2 * HD : 0));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int ps_shift = p.pages.ps_shift, n_kv = p.pages.n_kv, G = p.group;
-    const uint32_t total = pa_prefix<PA_THREADS>(p.seqs, ps_shift, n_kv, G, p.max_rows, ROWS, BLOCK, pre, warp_tot,
-                                                 blockIdx.x == 0 ? p.err : nullptr, p.alone != 0);
-    const PaDeal deal(total, gridDim.x);
-    const uint32_t x0 = deal.begin(blockIdx.x), x1 = deal.begin(blockIdx.x + 1);
-    pdl_launch_dependents();
-    if (x0 >= x1) return;
 
-    struct Cursor {  // a block of the line
+    struct Cursor {  // a block of keys of an item
         int s, item, b;
         PaWork w;
     };
-    auto at = [&](uint32_t x) {
-        Cursor c;
-        c.s = pa_find(pre, p.seqs.n_seqs, x);
-        c.w = pa_work(p.seqs, ps_shift, n_kv, G, p.max_rows, ROWS, BLOCK, c.s, nullptr);
-        const uint32_t y = x - pre[c.s];
-        c.item = (int)(y / (uint32_t)c.w.nb);
-        c.b = (int)(y % (uint32_t)c.w.nb);
-        return c;
-    };
-    auto next_item = [&](Cursor& c) {  // only called while blocks are left
+    auto work_of = [&](int s, int* err) { return pa_work(p.seqs, ps_shift, n_kv, G, p.max_rows, ROWS, BLOCK, s, err, p.alone != 0); };
+    Cursor f{}, end{};  // this CTA's first block, and the one after its last
+    if (CL == 1) {
+        const uint32_t total = pa_prefix<PA_THREADS>(p.seqs, ps_shift, n_kv, G, p.max_rows, ROWS, BLOCK, pre, warp_tot,
+                                                     blockIdx.x == 0 ? p.err : nullptr, p.alone != 0);
+        const PaDeal deal(total, gridDim.x);
+        const uint32_t x0 = deal.begin(blockIdx.x), x1 = deal.begin(blockIdx.x + 1);
+        pdl_launch_dependents();
+        if (x0 >= x1) return;
+        auto at = [&](uint32_t x) {  // the first block at or behind unit x
+            Cursor c;
+            c.s = pa_find(pre, p.seqs.n_seqs, x);
+            c.w = work_of(c.s, nullptr);
+            const uint32_t y = x - pre[c.s], u = c.w.units();
+            c.item = (int)(y / u);
+            c.b = max(0, (int)(y % u) - PA_ITEM);
+            return c;
+        };
+        f = at(x0);
+        if (x1 < total) end = at(x1);
+        else end.s = -1;
+    } else {
+        const int item = blockIdx.x / CL, rank = blockIdx.x % CL;
+        f.s = item / n_kv;
+        f.w = work_of(f.s, rank == 0 && item % n_kv == 0 ? p.err : nullptr);
+        if (f.w.items == 0) return;  // (the whole cluster)
+        f.item = item % n_kv;        // (one tile: max_rows is 16)
+        end = f;
+        f.b = (int)((long long)f.w.nb * rank / CL);
+        end.b = (int)((long long)f.w.nb * (rank + 1) / CL);
+    }
+    auto at_end = [&](const Cursor& c) { return c.s == end.s && c.item == end.item && c.b == end.b; };
+    auto next_item = [&](Cursor& c) {  // the next one's first block; behind the last item: s = -1, as in `end`
         c.b = 0;
         if (++c.item == c.w.items) {
             c.item = 0;
             do {
                 ++c.s;
-            } while (pre[c.s + 1] == pre[c.s]);
-            c.w = pa_work(p.seqs, ps_shift, n_kv, G, p.max_rows, ROWS, BLOCK, c.s, nullptr);
+            } while (c.s < p.seqs.n_seqs && pre[c.s + 1] == pre[c.s]);
+            if (c.s == p.seqs.n_seqs) c.s = -1;
+            else c.w = work_of(c.s, nullptr);
         }
     };
+    Cursor c = f;
 
     uint8_t* ring = smem + warp * PA_NS * SLOT;
     const uint32_t ring_u = smem_u32(ring);
-    Cursor f = at(x0);
-    uint32_t fx = x0;
+    bool more = !at_end(f);
+    // page table entries of the block to request next, read one request ahead (-2: past the sequence's end)
+    int entry[KEYS / 16];
+    auto look = [&]() {
+#pragma unroll
+        for (int part = 0; part < KEYS / 16; ++part) {
+            const int r0 = f.b * BLOCK + warp * KEYS + 16 * part;
+            entry[part] = more && r0 < f.w.kv ? p.seqs.table[(long long)f.s * p.seqs.max_pages + (r0 >> ps_shift)] : -2;
+        }
+    };
+    look();
     uint32_t dead = 0;  // slots (q8: half slots) whose page does not exist
     // Requests this warp's rows of the next block of the line into ring slot `slot`.
     auto fetch = [&](int slot) {
-        if (fx < x1) {
+        if (more) {
             const int h = f.item / f.w.tiles, k0 = f.b * BLOCK + warp * KEYS;
             const uint32_t dst = ring_u + slot * SLOT;
 #pragma unroll
             for (int part = 0; part < KEYS / 16; ++part) {  // sixteen rows lie in one page
                 const int r0 = k0 + 16 * part;
+                const int page = entry[part];
                 long long row = -1;
-                if (r0 < f.w.kv) row = page_row(p.pages, p.seqs, f.s, h, r0, lane == 0 ? p.err : nullptr);
+                if ((unsigned)page < (unsigned)p.pages.n_pages)
+                    row = page * p.pages.page_rows + h * p.pages.head_rows + (r0 & ((1 << ps_shift) - 1));
+                else if (page != -2 && lane == 0 && p.err)
+                    atomicOr(p.err, ERR_PAGE);
                 const uint32_t bit = 1u << (slot * 2 + part);
                 dead = row < 0 ? dead | bit : dead & ~bit;
                 const int left = row < 0 ? 0 : f.w.kv - r0;  // rows of the sequence from here on
@@ -271,20 +325,20 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
                     }
                 }
             }
-            ++fx;
-            if (++f.b == f.w.nb && fx < x1) next_item(f);
+            if (++f.b == f.w.nb && (CL == 1 || f.b != end.b)) next_item(f);
+            more = !at_end(f);
+            look();
         }
         cp_async_commit();
     };
 #pragma unroll
     for (int i = 0; i < PA_NS; ++i) fetch(i);
 
-    Cursor c = at(x0);
-    uint32_t x = x0;
     int slot = 0;
-    while (x < x1) {
+    bool again = CL > 1 || !at_end(c);  // (a CTA of a cluster without a block still takes part in the join)
+    while (again) {
         const int h = c.item / c.w.tiles, tile = c.item - h * c.w.tiles;
-        const int b0 = c.b, b1 = (int)min((uint32_t)c.w.nb, c.b + (x1 - x));
+        const int b0 = c.b, b1 = c.s == end.s && c.item == end.item ? end.b : c.w.nb;
         // this lane's rows g and g + 8 of every sixteen: last visible positions
         const int rows = c.w.n * G;
         auto q_row = [&](int r) {  // row r of the item (rows past the end: the last one, never stored)
@@ -525,6 +579,8 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
         // c4 ^ 2 ((c4 >> 3) & 3) ^ (r & 1))
         float* mine = reinterpret_cast<float*>(ring + slot * SLOT);
         const bool whole = b0 == 0 && b1 == c.w.nb;
+        if (CL > 1) cp_async_wait<0>();  // (nothing more was requested; the next slot of warp 0 takes this CTA's part)
+        float* part_c = reinterpret_cast<float*>(smem + (slot + 1 == PA_NS ? 0 : slot + 1) * SLOT);
         float* pt = p.part + (size_t)(2 * blockIdx.x + (b0 == 0 ? 1 : 0)) * PA_PART;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
@@ -589,7 +645,9 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
                         }
                         y[4 * e] = a.x; y[4 * e + 1] = a.y; y[4 * e + 2] = a.z; y[4 * e + 3] = a.w;
                     }
-                    if (whole) {
+                    if (CL > 1) {
+                        store8<float>(part_c + r * HD + col, y);
+                    } else if (whole) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) y[e] *= il;
                         store8<T>(dst + col, y);
@@ -597,17 +655,58 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
                         store8<float>(pt + rt * HD + col, y);
                     }
                 }
-                if (!whole && (tid & 7) == 0) {
+                if (CL > 1 && (tid & 7) == 0) {
+                    ml_c[0][rt] = mm;
+                    ml_c[1][rt] = ll;
+                }
+                if (CL == 1 && !whole && (tid & 7) == 0) {
                     pt[PA_ROWS_MAX * HD + rt] = mm;
                     pt[PA_ROWS_MAX * HD + PA_ROWS_MAX + rt] = ll;
                 }
             }
         }
+        if (CL > 1) {
+            // every CTA's part is in its own shared memory: CTA `rank` folds columns [16 rank, 16 rank + 16) of all
+            cluster_barrier();
+            const int r = tid >> 3, rr = tile * ROWS + r, rank = blockIdx.x % CL;
+            const int col = (HD / CL) * rank + 2 * (tid & 7);
+            if (rr < rows) {
+                float pm[CL], pl[CL], px[CL], py[CL];
+#pragma unroll
+                for (int k = 0; k < CL; ++k) {
+                    pm[k] = ld_cluster(&ml_c[0][r], k);
+                    pl[k] = ld_cluster(&ml_c[1][r], k);
+                    // (the slot that holds a CTA's part depends on how many blocks it had)
+                    const int n = (int)((long long)c.w.nb * (k + 1) / CL) - (int)((long long)c.w.nb * k / CL);
+                    const int sl = (max(n - 1, 0) + 1) % PA_NS;
+                    const float* pk = reinterpret_cast<const float*>(smem + sl * SLOT) + r * HD + col;
+                    px[k] = ld_cluster(pk, k);
+                    py[k] = ld_cluster(pk + 1, k);
+                }
+                float mm = pm[0];
+#pragma unroll
+                for (int k = 1; k < CL; ++k) mm = fmaxf(mm, pm[k]);
+                float ll = 0.f, ax = 0.f, ay = 0.f;
+#pragma unroll
+                for (int k = 0; k < CL; ++k) {
+                    const float fk = pm[k] == -INFINITY ? 0.f : ex2_approx(pm[k] - mm);
+                    ll = fmaf(fk, pl[k], ll);
+                    ax = fmaf(fk, px[k], ax);
+                    ay = fmaf(fk, py[k], ay);
+                }
+                const float il = mm == -INFINITY ? 0.f : 1.0f / ll;
+                T* dst = reinterpret_cast<T*>(p.out) + (c.w.q0 + rr / G) * p.out_stride + (h * G + rr % G) * HD + col;
+                *reinterpret_cast<uint32_t*>(dst) = pack_f<T>(ax * il, ay * il);
+            }
+            cluster_barrier();  // (no CTA leaves while its part is being read)
+            return;
+        }
         __syncthreads();
         fetch(slot);
         slot = slot + 1 == PA_NS ? 0 : slot + 1;
-        x += b1 - b0;
-        if (x < x1) next_item(c);
+        c.b = b1;
+        if (b1 == c.w.nb) next_item(c);
+        again = !at_end(c);
     }
     cp_async_wait<0>();
 }
@@ -630,8 +729,8 @@ __global__ void __launch_bounds__(512) paged_attn_join_kernel(const PagedAttnPar
     if (x0 >= x1) return;
     const int s = pa_find(pre, p.seqs.n_seqs, x1 - 1);
     const PaWork w = pa_work(p.seqs, p.pages.ps_shift, p.pages.n_kv, G, p.max_rows, ROWS, BLOCK, s, nullptr);
-    const uint32_t item = (x1 - 1 - pre[s]) / w.nb, i0 = pre[s] + item * w.nb, i1 = i0 + w.nb;
-    if (i0 < x0 || i1 <= x1) return;
+    const uint32_t u = w.units(), item = (x1 - 1 - pre[s]) / u, i0 = pre[s] + item * u, i1 = i0 + u;
+    if (i0 + PA_ITEM < x0 || i0 + PA_ITEM >= x1 || i1 <= x1) return;  // its first block is another CTA's, or its last is ours
     const int n_parts = (int)(deal.cta_of(i1 - 1) - c0) + 1;
     const int h = item / w.tiles, tile = item % w.tiles, rows = min(ROWS, w.n * G - tile * ROWS);
     int log_r = 0;  // rows in a round, a power of two up to 16; W = 16 >> log_r warps a row
