@@ -163,14 +163,14 @@ cudaError_t launch_attn(const PagedAttnParams& p, int dev, cudaStream_t st) {
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(512);
+    cfg.blockDim = dim3(PJ_WARPS * 32);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<T, 16 * MT, pa_block(Q8)>, p, ctas);
+    return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<T>, p);
 }
 
 // One cluster per (sequence, kv head), one launch.
@@ -244,7 +244,7 @@ cudaError_t launch_attn_tc(const PagedTcParams& p, int tiles, int dev, cudaStrea
     return cudaLaunchKernelEx(&cfg, paged_attn_tc_join_kernel<T>, p);
 }
 
-constexpr size_t PA_SCRATCH = (size_t)PA_MAX_CTAS * 2 * PA_PART * sizeof(float);
+constexpr size_t PA_SCRATCH = PA_MAX_CTAS * (2 * PA_PART * sizeof(float) + sizeof(PaSplit));
 constexpr size_t PC_SCRATCH = (size_t)PC_MAX_SHARES * PC_PART * sizeof(float);
 
 icua_status check_attn(const icua_kv_pages* pages, const icua_kv_seqs* seqs, int32_t n_q, PagesView* P, SeqsView* S) {
@@ -359,6 +359,7 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
     p.scale_log2 = (a->scale > 0.f ? a->scale : 0.08838834764831845f) * 1.4426950408889634f;
     p.max_rows = PA_ROWS_FEW;
     p.part = (float*)a->scratch;
+    p.split = (PaSplit*)(p.part + (size_t)PA_MAX_CTAS * 2 * PA_PART);
     p.err = err_dev;
     cudaStream_t s = (cudaStream_t)stream;
     const bool f16 = a->dtype == ICUA_DT_F16, q8 = pages->dtype == ICUA_KV_Q8;

@@ -19,8 +19,10 @@
 // * q8 rows are converted in registers, exactly: code -> 16-bit float by placing the byte in the
 //   mantissa of 1024 (fp16) or 128 / 256 (bf16) and subtracting.  The scales never round anything: the
 //   K scale multiplies the fp32 score; the V scale enters the exponent, p' = 2^(s + log2 vs - m') with
-//   m' the running maximum of that sum, so the 16-bit operand of the P V product lies in [0, 1] whatever
+//   m' the running maximum of that sum, so the 16-bit operand of the P V product lies in [0, 256] whatever
 //   the scales are, and the row sum is l = sum p' / vs.
+// The running maximum is only moved (and the output rescaled) when a score exceeds it by more than 2^8: the
+// rescale is then rare, and p below 256 is as precise in 16 bits as p below 1.
 // Scores, maxima, sums and outputs are fp32; p is rounded once to the 16-bit type of q.
 #pragma once
 #include "paged.cuh"
@@ -36,6 +38,13 @@ constexpr int PA_ITEM = 2;
 constexpr int PA_CLUSTER = 8;     // CTAs that share an item in the small-batch form
 constexpr int PA_MAX_CTAS = 320;  // workspace slots are laid out for so many
 constexpr int PA_MAX_SEQS = 1024;
+// What a CTA leaves for the join: the item that it began and did not end.
+struct PaSplit {
+    int n_parts;  // CTAs that worked on it (0: nothing to join), this one first
+    int first, rows;  // the tile's first row among the sequence's, its rows
+    int q0, h;
+    int pad[3];
+};
 constexpr int PA_PART = PA_ROWS_MAX * HD + 2 * PA_ROWS_MAX;  // floats of a part: o[32][128], m[32], l[32]
 
 struct PagedAttnParams {
@@ -49,6 +58,7 @@ struct PagedAttnParams {
     int max_rows;      // sequences with more rows (n G) than this belong to another kernel,
     int alone;         //   or, when there is none in this call, break the caller's max_q (ERR_SEQ)
     float* part;       // [gridDim.x][2][PA_PART]: 0 = an item begun by an earlier CTA, 1 = an item begun here
+    PaSplit* split;    // [gridDim.x]
     int* err;
 };
 
@@ -74,6 +84,9 @@ __device__ __forceinline__ float ld_cluster(const float* here, uint32_t rank) {
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -224,6 +237,21 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
                                                      blockIdx.x == 0 ? p.err : nullptr, p.alone != 0);
         const PaDeal deal(total, gridDim.x);
         const uint32_t x0 = deal.begin(blockIdx.x), x1 = deal.begin(blockIdx.x + 1);
+        // the item of this CTA's last unit is its to be joined when its first block is here and its end is not
+        PaSplit sp{};
+        if (x0 < x1) {
+            const int s = pa_find(pre, p.seqs.n_seqs, x1 - 1);
+            const PaWork w = work_of(s, nullptr);
+            const uint32_t u = w.units(), item = (x1 - 1 - pre[s]) / u, i0 = pre[s] + item * u, i1 = i0 + u;
+            if (i0 + PA_ITEM >= x0 && i0 + PA_ITEM < x1 && i1 > x1) {
+                sp.n_parts = (int)(deal.cta_of(i1 - 1) - blockIdx.x) + 1;
+                sp.h = item / w.tiles;
+                sp.first = (item % w.tiles) * ROWS;
+                sp.rows = min(ROWS, w.n * G - sp.first);
+                sp.q0 = w.q0;
+            }
+        }
+        if (tid == 0) p.split[blockIdx.x] = sp;
         pdl_launch_dependents();
         if (x0 >= x1) return;
         auto at = [&](uint32_t x) {  // the first block at or behind unit x
@@ -294,27 +322,43 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
                 dead = row < 0 ? dead | bit : dead & ~bit;
                 const int left = row < 0 ? 0 : f.w.kv - r0;  // rows of the sequence from here on
                 const long long base = row < 0 ? 0 : row;
+                // (sixteen rows lie in one page, so a row behind the sequence's end still has an address; it is not read)
+                const uint8_t *ks = p.pages.k + base * ROW + lane * 16, *vs = p.pages.v + base * ROW + lane * 16;
                 if (!Q8) {
-                    const uint8_t *ks = p.pages.k + base * ROW + lane * 16, *vs = p.pages.v + base * ROW + lane * 16;
+                    const uint32_t d = dst + lane * 16;
+                    if (left >= 16) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const bool real = 2 * i + (lane >> 4) < left;
-                        cp_async16(dst + i * 512 + lane * 16, real ? ks + i * 512 : p.pages.k, real);
-                        cp_async16(dst + KEYS * ROW + i * 512 + lane * 16, real ? vs + i * 512 : p.pages.v, real);
+                        for (int i = 0; i < 8; ++i) {
+                            cp_async16(d + i * 512, ks + i * 512);
+                            cp_async16(d + KEYS * ROW + i * 512, vs + i * 512);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const bool real = 2 * i + (lane >> 4) < left;
+                            cp_async16(d + i * 512, ks + i * 512, real);
+                            cp_async16(d + KEYS * ROW + i * 512, vs + i * 512, real);
+                        }
                     }
                 } else {
                     // chunk c of row r goes to c ^ 4 (r & 1) for K and c ^ 2 ((r >> 1) & 3) for V: the places that
                     // make the fragment reads below free of bank conflicts
-                    const int c = lane & 7;
+                    const int c = lane & 7, q = lane >> 3;
+                    const uint32_t dk = dst + (16 * part + q) * ROW + ((c ^ ((q & 1) << 2)) << 4);
+                    const uint32_t dv = dst + (KEYS + 16 * part + q) * ROW + ((c ^ ((q >> 1) << 1)) << 4);
+                    if (left >= 16) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = 4 * i + (lane >> 3);
-                        const bool real = r < left;
-                        const uint32_t at_row = dst + (16 * part + r) * ROW;
-                        const long long off = (base + r) * ROW + c * 16;
-                        cp_async16(at_row + ((c ^ ((r & 1) << 2)) << 4), real ? p.pages.k + off : p.pages.k, real);
-                        cp_async16(at_row + KEYS * ROW + ((c ^ (((r >> 1) & 3) << 1)) << 4), real ? p.pages.v + off : p.pages.v,
-                                   real);
+                        for (int i = 0; i < 4; ++i) {  // rows 4 i + q
+                            cp_async16(dk + i * 512, ks + i * 512);
+                            cp_async16((dv ^ ((i & 1) << 6)) + i * 512, vs + i * 512);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool real = 4 * i + q < left;
+                            cp_async16(dk + i * 512, ks + i * 512, real);
+                            cp_async16((dv ^ ((i & 1) << 6)) + i * 512, vs + i * 512, real);
+                        }
                     }
                     if (lane < 8) {  // scales: a quad that reaches past the sequence's end is read whole (same page)
                         const int e = (lane & 3) * 4;
@@ -507,9 +551,9 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
                         for (int nt = 1; nt < NT; ++nt) bm = fmaxf(bm, fmaxf(s[mt][nt][2 * i], s[mt][nt][2 * i + 1]));
                         bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
                         bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
-                        mn[i] = fmaxf(m[mt][i], bm);
+                        mn[i] = bm > m[mt][i] + 8.f ? bm : m[mt][i];
                     }
-                    if (__any_sync(0xffffffffu, mn[0] > m[mt][0] || mn[1] > m[mt][1])) {
+                    if (__any_sync(0xffffffffu, mn[0] != m[mt][0] || mn[1] != m[mt][1])) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const float corr = m[mt][i] == -INFINITY ? 0.f : ex2_approx(m[mt][i] - mn[i]);
@@ -711,46 +755,36 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
     cp_async_wait<0>();
 }
 
-// Folds the parts of the items that more than one CTA of paged_attn_kernel (grid `ctas`, the same
-// arguments) worked on.  CTA c takes the item that c began and did not end.  Sixteen warps: with few rows
-// several warps share one (each takes every W-th part, eight in flight) and meet in shared memory; the
-// grouping depends on the sizes alone, so the bits do too.
-template <typename T, int ROWS, int BLOCK>
-__global__ void __launch_bounds__(512) paged_attn_join_kernel(const PagedAttnParams p, int ctas) {
-    __shared__ uint32_t pre[PA_MAX_SEQS + 1];
-    __shared__ uint32_t warp_tot[16];
-    __shared__ float4 acc_s[16][32];
-    __shared__ float ml_s[16][2];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = p.group;
-    const uint32_t total =
-        pa_prefix<512>(p.seqs, p.pages.ps_shift, p.pages.n_kv, G, p.max_rows, ROWS, BLOCK, pre, warp_tot, nullptr);
-    const PaDeal deal(total, ctas);
-    const uint32_t c0 = blockIdx.x, x0 = deal.begin(c0), x1 = deal.begin(c0 + 1);
-    if (x0 >= x1) return;
-    const int s = pa_find(pre, p.seqs.n_seqs, x1 - 1);
-    const PaWork w = pa_work(p.seqs, p.pages.ps_shift, p.pages.n_kv, G, p.max_rows, ROWS, BLOCK, s, nullptr);
-    const uint32_t u = w.units(), item = (x1 - 1 - pre[s]) / u, i0 = pre[s] + item * u, i1 = i0 + u;
-    if (i0 + PA_ITEM < x0 || i0 + PA_ITEM >= x1 || i1 <= x1) return;  // its first block is another CTA's, or its last is ours
-    const int n_parts = (int)(deal.cta_of(i1 - 1) - c0) + 1;
-    const int h = item / w.tiles, tile = item % w.tiles, rows = min(ROWS, w.n * G - tile * ROWS);
-    int log_r = 0;  // rows in a round, a power of two up to 16; W = 16 >> log_r warps a row
-    while (log_r < 4 && (1 << log_r) < rows) ++log_r;
-    const int W = 16 >> log_r, piece = warp >> log_r;
+// Folds the parts of the items that more than one CTA of paged_attn_kernel worked on: CTA c takes the item
+// that c began and did not end.  Eight warps: with few rows several warps share one (each takes every W-th
+// part, eight in flight) and meet in shared memory; the grouping depends on the sizes alone, so the bits do
+// too.
+constexpr int PJ_WARPS = 8;
+template <typename T>
+__global__ void __launch_bounds__(PJ_WARPS * 32) paged_attn_join_kernel(const PagedAttnParams p) {
+    __shared__ float4 acc_s[PJ_WARPS][32];
+    __shared__ float ml_s[PJ_WARPS][2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.group;
     pdl_wait();
-    for (int r0 = 0; r0 < rows; r0 += 1 << log_r) {
+    const PaSplit sp = p.split[blockIdx.x];
+    if (sp.n_parts == 0) return;
+    int log_r = 0;  // rows in a round, a power of two; W warps a row
+    while (log_r < 3 && (1 << log_r) < sp.rows) ++log_r;
+    const int W = PJ_WARPS >> log_r, piece = warp >> log_r;
+    for (int r0 = 0; r0 < sp.rows; r0 += 1 << log_r) {
         const int r = r0 + (warp & ((1 << log_r) - 1));
         float m = -INFINITY, l = 0.f;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < rows) {
-            for (int k0 = piece; k0 < n_parts; k0 += 8 * W) {
+        if (r < sp.rows) {
+            for (int k0 = piece; k0 < sp.n_parts; k0 += 8 * W) {
                 float pm[8], pl[8];
                 float4 v[8];
 #pragma unroll
                 for (int u = 0; u < 8; ++u) {
                     const int k = k0 + u * W;
                     pm[u] = -INFINITY;
-                    if (k < n_parts) {
-                        const float* pt = p.part + (size_t)(2 * (c0 + k) + (k == 0 ? 1 : 0)) * PA_PART;
+                    if (k < sp.n_parts) {
+                        const float* pt = p.part + (size_t)(2 * (blockIdx.x + k) + (k == 0 ? 1 : 0)) * PA_PART;
                         pm[u] = pt[PA_ROWS_MAX * HD + r];
                         pl[u] = pt[PA_ROWS_MAX * HD + PA_ROWS_MAX + r];
                         v[u] = *reinterpret_cast<const float4*>(pt + r * HD + 4 * lane);
@@ -775,7 +809,7 @@ __global__ void __launch_bounds__(512) paged_attn_join_kernel(const PagedAttnPar
                     }
             }
         }
-        if (W > 1) {
+        if (W > 1) {  // (one round: the rows are fewer than the warps)
             acc_s[warp][lane] = a;
             if (lane == 0) {
                 ml_s[warp][0] = m;
@@ -797,10 +831,10 @@ __global__ void __launch_bounds__(512) paged_attn_join_kernel(const PagedAttnPar
                     a.w = a.w * f0 + v.w * f1;
                 }
         }
-        if (piece == 0 && r < rows) {
+        if (piece == 0 && r < sp.rows) {
             const float il = m == -INFINITY ? 0.f : 1.0f / l;
-            const int rr = tile * ROWS + r;
-            T* dst = reinterpret_cast<T*>(p.out) + (w.q0 + rr / G) * p.out_stride + (h * G + rr % G) * HD + 4 * lane;
+            const int rr = sp.first + r;
+            T* dst = reinterpret_cast<T*>(p.out) + (sp.q0 + rr / G) * p.out_stride + (sp.h * G + rr % G) * HD + 4 * lane;
             *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f<T>(a.x * il, a.y * il), pack_f<T>(a.z * il, a.w * il));
         }
     }
