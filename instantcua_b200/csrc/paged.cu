@@ -158,7 +158,7 @@ cudaError_t launch_attn(const PagedAttnParams& p, int dev, cudaStream_t st) {
     const int smem = pa_smem(Q8, MT, 1);
     cudaError_t e = allow_smem<paged_attn_kernel<T, Q8, MT, 1>>(smem, dev);
     if (e != cudaSuccess) return e;
-    const int ctas = std::min(PA_MAX_CTAS, 2 * sm_count(dev));
+    const int ctas = std::min(PA_MAX_CTAS, pa_ctas(Q8, MT) * sm_count(dev));
     paged_attn_kernel<T, Q8, MT, 1><<<ctas, PA_THREADS, smem, st>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};

@@ -8,11 +8,11 @@
 // head), the M of mma.sync.m16n8k16, so every K/V byte is read once for all rows of the tile.
 //
 // Bound: HBM (4 G FLOP per cached byte and row).  What follows from it:
-// * The items' blocks (64 keys, 128 in a q8 cache) are dealt evenly over the CTAs, two per SM, as one
+// * The items' blocks (64 keys, 128 in a q8 cache) are dealt evenly over the CTAs, two or three per SM, as one
 //   line: by the real lengths, read on the device, so a batch of very different lengths leaves no SM
 //   idle.  A CTA that holds a part of an item writes (max, sum, output) to the workspace, and
 //   paged_attn_join_kernel folds an item's parts in the order of their keys: the same bits every run.
-// * Each of the four warps streams its own sixteen (q8: 32) rows of a block through a ring of three
+// * Each of the four warps streams its own sixteen (q8: 32) rows of a block through a ring of two or three
 //   slots with 16-byte cp.async, and runs its own online softmax; only the end of an item meets in
 //   shared memory.  Rows behind the sequence's end are never read: cp.async fills zeros, so whatever a
 //   page still holds there (NaN included) cannot reach a sum.
@@ -33,10 +33,9 @@ namespace icua {
 constexpr int PA_ROWS_MAX = 32;   // query rows per item: 16 or 32
 constexpr int PA_WARPS = 4;
 constexpr int PA_THREADS = PA_WARPS * 32;
-constexpr int PA_NS = 3;          // ring slots per warp
 constexpr int PA_ITEM = 2;
 constexpr int PA_CLUSTER = 8;     // CTAs that share an item in the small-batch form
-constexpr int PA_MAX_CTAS = 320;  // workspace slots are laid out for so many
+constexpr int PA_MAX_CTAS = 480;  // workspace slots are laid out for so many
 constexpr int PA_MAX_SEQS = 1024;
 // What a CTA leaves for the join: the item that it began and did not end.
 struct PaSplit {
@@ -65,8 +64,14 @@ struct PagedAttnParams {
 constexpr int pa_keys(bool q8) { return q8 ? 32 : 16; }  // rows of a warp's slot
 constexpr int pa_block(bool q8) { return PA_WARPS * pa_keys(q8); }
 constexpr int pa_slot(bool q8) { return q8 ? 32 * 2 * HD + 2 * 32 * 4 : 16 * 2 * HD * 2; }
+// CTAs per SM and ring slots per warp.  Sixteen rows of a q8 cache: three CTAs (their fragments' conversion is
+// a chain of dependent instructions, which more warps hide), with the q fragments in shared memory to fit the
+// registers.  Else two, which stream a 16-bit cache at HBM speed.
+constexpr int pa_ctas(bool q8, int mt) { return q8 && mt == 1 ? 3 : 2; }
+constexpr int pa_ns(bool q8, int mt) { return pa_ctas(q8, mt) == 3 ? 2 : 3; }
+constexpr bool pa_q_in_smem(bool q8, int mt) { return mt > 1 || q8; }
 constexpr int pa_smem(bool q8, int mt, int cl) {
-    return PA_WARPS * PA_NS * pa_slot(q8) + (mt > 1 ? mt * 16 * 2 * HD : 0) + (cl > 1 ? 0 : (PA_MAX_SEQS + 1) * 4);
+    return PA_WARPS * pa_ns(q8, mt) * pa_slot(q8) + (pa_q_in_smem(q8, mt) ? mt * 16 * 2 * HD : 0) + (cl > 1 ? 0 : (PA_MAX_SEQS + 1) * 4);
 }
 
 __device__ __forceinline__ void cluster_barrier() {
@@ -214,15 +219,17 @@ struct PaDeal {
 // head) of the cluster's number, and join its parts through distributed shared memory.  One launch and no
 // workspace, for calls whose time is latency.
 template <typename T, bool Q8, int MT, int CL>
-__global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(PA_THREADS, pa_ctas(Q8, MT)) paged_attn_kernel(const PagedAttnParams p) {
+    constexpr int PA_NS = pa_ns(Q8, MT);
+    constexpr bool QS = pa_q_in_smem(Q8, MT);
     constexpr int KEYS = pa_keys(Q8), BLOCK = pa_block(Q8), SLOT = pa_slot(Q8), NT = KEYS / 8, ROWS = 16 * MT;
     constexpr int ROW = Q8 ? HD : 2 * HD;  // bytes of a cached row
-    extern __shared__ __align__(1024) uint8_t smem[];
+    extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float ml[PA_WARPS][2][ROWS];
     __shared__ float ml_c[2][ROWS];  // CL > 1: this CTA's part's
     __shared__ uint32_t warp_tot[PA_WARPS];
-    uint8_t* q_tile = smem + PA_WARPS * PA_NS * SLOT;  // MT > 1: the rows of the item, 256 B each, chunk c at c ^ (row & 7)
-    uint32_t* pre = reinterpret_cast<uint32_t*>(q_tile + (MT > 1 ? ROWS * 2 * HD : 0));
+    uint8_t* q_tile = smem + PA_WARPS * PA_NS * SLOT;  // QS: the rows of the item, 256 B each, chunk c at c ^ (row & 7)
+    uint32_t* pre = reinterpret_cast<uint32_t*>(q_tile + (QS ? ROWS * 2 * HD : 0));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int ps_shift = p.pages.ps_shift, n_kv = p.pages.n_kv, G = p.group;
 
@@ -395,26 +402,20 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int r = tile * ROWS + 16 * mt + g + 8 * i;
-                lim[mt][i] = r < rows ? c.w.kv - c.w.n + r / G : -1;
+                lim[mt][i] = c.w.kv - c.w.n + min(r, rows - 1) / G;  // (rows past the end: the last one's)
             }
         // A fragments of q.  In a q8 cache a lane's K codes are 32-bit words of four dimensions d0 .. d0 + 3, used
         // as the pairs (d0, d0 + 2) and (d0 + 1, d0 + 3), so q takes the same order: word 2 t + 16 ks of a row
         // holds the first pair of d0 = 64 (ks / 4) + 16 t + 4 (ks % 4), word 2 t + 16 ks + 8 the second.
-        uint32_t qa[MT == 1 ? 8 : 1][4];
-        if (MT == 1) {
+        uint32_t qa[QS ? 1 : 8][4];
+        if (!QS) {
             const T* qp[2] = {q_row(g), q_row(g + 8)};
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    if (!Q8) {
-                        qa[ks][i] = *reinterpret_cast<const uint32_t*>(qp[i] + 16 * ks + 2 * t);
-                        qa[ks][2 + i] = *reinterpret_cast<const uint32_t*>(qp[i] + 16 * ks + 2 * t + 8);
-                    } else {
-                        const uint2 v = *reinterpret_cast<const uint2*>(qp[i] + 64 * (ks >> 2) + 16 * t + 4 * (ks & 3));
-                        qa[ks][i] = prmt(v.x, v.y, 0x5410);
-                        qa[ks][2 + i] = prmt(v.x, v.y, 0x7632);
-                    }
+                    qa[QS ? 0 : ks][i] = *reinterpret_cast<const uint32_t*>(qp[i] + 16 * ks + 2 * t);
+                    qa[QS ? 0 : ks][2 + i] = *reinterpret_cast<const uint32_t*>(qp[i] + 16 * ks + 2 * t + 8);
                 }
         } else {
             // (the barriers at the end of an item are behind every read of the tile before)
@@ -438,9 +439,9 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
         }
         const uint32_t q_u = smem_u32(q_tile);
         auto q_frag = [&](int mt, int ks, uint32_t (&a)[4]) {
-            if (MT == 1) {
+            if (!QS) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = qa[MT == 1 ? ks : 0][i];
+                for (int i = 0; i < 4; ++i) a[i] = qa[QS ? 0 : ks][i];
             } else {  // rows 0-7 / 8-15 of chunk 2 ks, then of 2 ks + 1
                 const int r = 16 * mt + (lane & 15);
                 ldsm_x4(a, q_u + r * 256 + (((2 * ks + (lane >> 4)) ^ (r & 7)) << 4));
@@ -532,32 +533,47 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
 #pragma unroll
                             for (int e = 0; e < 4; ++e) s[mt][nt][e] *= p.scale_log2;
                 }
-                uint32_t pa[MT][NT / 2][4];
+                // Every step is taken for all tiles before the next one, and the two branches are uniform: the tiles'
+                // chains of dependent instructions overlap.
+                const uint32_t gone = (dead >> (2 * slot)) & 3u;
+                int low = lim[0][0];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    const uint32_t gone = dead >> (2 * slot);
-                    if (gone & 3u || __any_sync(0xffffffffu, k0 + KEYS - 1 > min(lim[mt][0], lim[mt][1]))) {
+                for (int mt = 0; mt < MT; ++mt) low = min(low, min(lim[mt][0], lim[mt][1]));
+                if (gone || __any_sync(0xffffffffu, k0 + KEYS - 1 > low)) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
                                 if (k0 + 8 * nt + 2 * t + (e & 1) > lim[mt][e >> 1] || (gone >> (nt >> 1)) & 1u) s[mt][nt][e] = -INFINITY;
-                    }
-                    float mn[2];
+                }
+                float bm[MT][2];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float bm = fmaxf(s[mt][0][2 * i], s[mt][0][2 * i + 1]);
+                        bm[mt][i] = fmaxf(s[mt][0][2 * i], s[mt][0][2 * i + 1]);
 #pragma unroll
-                        for (int nt = 1; nt < NT; ++nt) bm = fmaxf(bm, fmaxf(s[mt][nt][2 * i], s[mt][nt][2 * i + 1]));
-                        bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
-                        bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
-                        mn[i] = bm > m[mt][i] + 8.f ? bm : m[mt][i];
+                        for (int nt = 1; nt < NT; ++nt) bm[mt][i] = fmaxf(bm[mt][i], fmaxf(s[mt][nt][2 * i], s[mt][nt][2 * i + 1]));
                     }
-                    if (__any_sync(0xffffffffu, mn[0] != m[mt][0] || mn[1] != m[mt][1])) {
+#pragma unroll
+                for (int x = 1; x < 4; x <<= 1)
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) bm[mt][i] = fmaxf(bm[mt][i], __shfl_xor_sync(0xffffffffu, bm[mt][i], x));
+                bool move = false;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) move |= bm[mt][0] > m[mt][0] + 8.f || bm[mt][1] > m[mt][1] + 8.f;
+                if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const float corr = m[mt][i] == -INFINITY ? 0.f : ex2_approx(m[mt][i] - mn[i]);
-                            m[mt][i] = mn[i];
+                            const float mn = bm[mt][i] > m[mt][i] + 8.f ? bm[mt][i] : m[mt][i];
+                            const float corr = m[mt][i] == -INFINITY ? 0.f : ex2_approx(m[mt][i] - mn);
+                            m[mt][i] = mn;
                             l[mt][i] *= corr;
 #pragma unroll
                             for (int j = 0; j < 16; ++j) {
@@ -565,7 +581,10 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
                                 o[mt][j][2 * i + 1] *= corr;
                             }
                         }
-                    }
+                }
+                uint32_t pa[MT][NT / 2][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const float ms = m[mt][i] == -INFINITY ? 0.f : m[mt][i];
@@ -576,7 +595,6 @@ __global__ void __launch_bounds__(PA_THREADS, 2) paged_attn_kernel(const PagedAt
                             pa[mt][nt >> 1][2 * (nt & 1) + i] = pack_f<T>(e0, e1);
                         }
                     }
-                }
                 if (!Q8) {
                     const int row = (lane & 7) + (((lane >> 3) & 1) << 3);
 #pragma unroll
