@@ -68,6 +68,10 @@ icua_status check_cache(const icua_kv_pages* c, const icua_kv_seqs* s, PagesView
     }
     if (P->page_rows < c->page_size || P->page_rows % 16 || P->head_rows < c->page_size || P->head_rows % 16)
         return bad("page_rows and head_rows are multiples of 16, at least page_size (or both 0)");
+    // (the kernels count pool rows in 32 bits: 2^32 rows are 512 GB)
+    if (P->page_rows > UINT32_MAX || P->head_rows > UINT32_MAX ||
+        (double)c->n_pages * P->page_rows + (double)c->n_kv * P->head_rows > 4294967295.0)
+        return bad("the pool is too large");
     if (s->n_seqs > 0 && (!s->cu_q || !s->kv_len || (s->max_pages > 0 && !s->page_table))) return bad("null batch arrays");
     if (!aligned(s->cu_q, 4) || !aligned(s->kv_len, 4) || !aligned(s->page_table, 4)) return bad("batch arrays are not aligned");
     if ((int64_t)s->max_pages * c->page_size > INT32_MAX) return bad("max_pages * page_size is above 2^31 - 1");
@@ -113,18 +117,15 @@ cudaError_t allow_smem(int bytes, int dev) {
 int vectors_per_unit(int64_t tokens, int n_vec, int n_sm) { return tokens * ((n_vec + 3) / 4) >= 2ll * 16 * n_sm ? 4 : 1; }
 
 template <typename TI, typename TQ, int KVD>
-cudaError_t launch_write(KvWriteParams& p, int n_sm, cudaStream_t st) {
-    const int n_vec = p.n_q + 2 * p.pages.n_kv;
-    const int vpt = vectors_per_unit(p.seqs.total_q, n_vec, n_sm);
-    p.n_groups = (n_vec + vpt - 1) / vpt;
-    const int64_t grid = ((int64_t)p.seqs.total_q * p.n_groups + 15) / 16;
-    if (vpt == 4) kv_write_kernel<TI, TQ, KVD, 4><<<(unsigned)grid, 256, 0, st>>>(p);
-    else kv_write_kernel<TI, TQ, KVD, 1><<<(unsigned)grid, 256, 0, st>>>(p);
+cudaError_t launch_write(const KvWriteParams& p, int n_sm, cudaStream_t st) {
+    // four tokens a CTA once that leaves two CTAs per SM
+    if (p.seqs.total_q >= 8 * n_sm) kv_write_kernel<TI, TQ, KVD, 4><<<(p.seqs.total_q - 1) / 4 + 1, 256, 0, st>>>(p);
+    else kv_write_kernel<TI, TQ, KVD, 1><<<p.seqs.total_q, 256, 0, st>>>(p);
     return cudaGetLastError();
 }
 
 template <typename TI>
-cudaError_t launch_write_in(KvWriteParams& p, int kvd, int qd, int n_sm, cudaStream_t st) {
+cudaError_t launch_write_in(const KvWriteParams& p, int kvd, int qd, int n_sm, cudaStream_t st) {
     if (kvd == ICUA_KV_F16) return launch_write<TI, __half, KV_F16>(p, n_sm, st);
     if (kvd == ICUA_KV_BF16) return launch_write<TI, __nv_bfloat16, KV_BF16>(p, n_sm, st);
     return qd == ICUA_DT_F16 ? launch_write<TI, __half, KV_Q8>(p, n_sm, st) : launch_write<TI, __nv_bfloat16, KV_Q8>(p, n_sm, st);
@@ -281,7 +282,6 @@ icua_status icua_kv_write(const icua_kv_pages* pages, const icua_kv_seqs* seqs, 
         return bad("a row array is not aligned");
     if (rows->rope && rows->rope_len < 0) return bad("rope_len is negative");
     if (!(rows->eps >= 0.f)) return bad("eps is negative or NaN");
-    if ((int64_t)seqs->total_q * (rows->n_q + 2 * pages->n_kv) > ((int64_t)16 << 31) - 16) return bad("the batch is too large: split it");
     if (seqs->n_seqs == 0 || seqs->total_q == 0) return ICUA_OK;
     int dev = 0;
     if ((st = current(pages, rows->qkv, &dev)) != ICUA_OK) return st;

@@ -81,7 +81,6 @@ struct KvWriteParams {
     float eps;
     void* q_out;
     long long q_stride;
-    int n_groups;  // half-warps per token, each for VPT consecutive head vectors
     int* err;
 };
 
@@ -139,142 +138,205 @@ __device__ __forceinline__ void store8<float>(float* p, const float (&x)[8]) {
     reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
 
-// One half-warp per head vector, 16 lanes x 8 elements: y = x rsqrt(mean x^2 + eps) w, then the
-// rotation of the pairs (j, j + 64) (the partner's eight are eight lanes away), both in fp32; q rows
-// are rounded to the output type, k and v rows to the cache type or to int8 codes: scale = max|x| /
-// 127 in fp32 and code = x / scale to the nearest even, so a code is off by at most half a step.  A
-// row that holds a NaN or an infinity gets the scale NaN and reads back as NaN throughout.  A row
-// of zeros gets the scale 1.
-// Bound: HBM for many tokens (each row read once and written once), latency for few, so a half-warp
-// takes VPT = 4 consecutive vectors of a token (its loads issued together, the sequence lookup and
-// the rotation row shared) where that still fills the GPU and one otherwise.
-template <typename TI, typename TQ, int KVD, int VPT>
-__global__ void __launch_bounds__(256) kv_write_kernel(const KvWriteParams p) {
-    using TC = typename std::conditional<KVD == KV_BF16, __nv_bfloat16, __half>::type;
-    const int lane = threadIdx.x & 31, l = lane & 15;
-    const long long unit = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;
-    const int t = (int)(unit / p.n_groups), v0 = (int)(unit % p.n_groups) * VPT;
-    // both halves' tokens, looked up by the whole warp
-    const int ta = __shfl_sync(0xffffffffu, t, 0), tb = __shfl_sync(0xffffffffu, t, 16);
-    const int sa = find_seq(p.seqs, ta, lane);
-    const int sb = tb == ta ? sa : find_seq(p.seqs, tb, lane);
-    const int s = lane < 16 ? sa : sb;
-    const int n_kv = p.pages.n_kv, n_vec = p.n_q + 2 * n_kv;
-    bool live = t < p.seqs.total_q && s < p.seqs.n_seqs;
-    int pos = 0;
-    if (live) {
-        const SeqInfo q = load_seq(p.seqs, p.pages.ps_shift, s, l == 0 ? p.err : nullptr);
-        pos = q.kv - q.n + (t - q.q0);
-        live = t >= q.q0 && t < q.q0 + q.n;
-        if (live && pos < 0) {  // more new tokens than positions: this one has no place
-            live = false;
-            if (p.err && l == 0) atomicOr(p.err, ERR_SEQ);
+// Four consecutive elements as they lie in memory, as floats, and back.
+template <typename T>
+struct Raw4 {
+    typename std::conditional<sizeof(T) == 4, float4, uint2>::type v;
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const decltype(v)*>(p); }
+};
+template <typename T>
+__device__ __forceinline__ void unpack4(const Raw4<T>& raw, float* x) {
+    if constexpr (sizeof(T) == 4) {
+        x[0] = raw.v.x; x[1] = raw.v.y; x[2] = raw.v.z; x[3] = raw.v.w;
+    } else {
+        const uint32_t w[2] = {raw.v.x, raw.v.y};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                x[2 * i] = f.x;
+                x[2 * i + 1] = f.y;
+            } else {
+                x[2 * i] = __uint_as_float(w[i] << 16);
+                x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
         }
     }
-    float cs[8], sn[8];
+}
+__device__ __forceinline__ void load4(const float* p, float* x) {
+    Raw4<float> raw;
+    raw.load(p);
+    unpack4(raw, x);
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const float* x) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_f<T>(x[0], x[1]), pack_f<T>(x[2], x[3]));
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// A half-warp per head vector: lane l holds elements 4 l .. 4 l + 3 and 64 + 4 l .., the two halves of four
+// rotation pairs.  y = x rsqrt(mean x^2 + eps) w, then (y_j c - y_{j+64} s, y_{j+64} c + y_j s), in fp32; q rows
+// are rounded to the output type, k and v rows to the cache type or to int8 codes: scale = max|x| / 127 in fp32
+// and code = x / scale to the nearest even, so a code is off by at most half a step.  A row that holds a NaN
+// or an infinity gets the scale NaN and reads back as NaN throughout.  A row of zeros gets the scale 1.
+// A CTA takes TOK tokens: a warp each looks its sequence, position and page up, then every token's vectors
+// are dealt to 16 / TOK half-warps, each with its token's rotation row and the norm weights in registers and
+// four vectors' loads in flight.  Bound: HBM for many tokens (each row is read once and written once; TOK = 4
+// shares the lookups), latency for few (TOK = 1).
+template <typename TI, typename TQ, int KVD, int TOK>
+__global__ void __launch_bounds__(256, sizeof(TI) == 4 ? 3 : 4) kv_write_kernel(const KvWriteParams p) {
+    using TC = typename std::conditional<KVD == KV_BF16, __nv_bfloat16, __half>::type;
+    constexpr int U = 4, STEP = 16 / TOK;
+    struct Token {
+        long long row;  // pool row of kv head 0, -1: no page
+        int pos, rope;  // rope: -1 = the token is left out
+    };
+    __shared__ Token tok_s[TOK];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & 15;
+    const int n_kv = p.pages.n_kv, n_vec = p.n_q + 2 * n_kv;
+    if (warp < TOK) {
+        const int t = blockIdx.x * TOK + warp;
+        const int s = t < p.seqs.total_q ? find_seq(p.seqs, t, lane) : p.seqs.n_seqs;
+        if (lane == 0) {
+            Token k{-1, 0, -1};
+            if (s < p.seqs.n_seqs) {
+                const SeqInfo q = load_seq(p.seqs, p.pages.ps_shift, s, p.err);
+                k.pos = q.kv - q.n + (t - q.q0);
+                if (t >= q.q0 && t < q.q0 + q.n) {
+                    const int r = p.rope == nullptr ? 0 : p.rope_rows != nullptr ? p.rope_rows[t] : k.pos;
+                    if (k.pos < 0 || (p.rope != nullptr && (unsigned)r >= (unsigned)p.rope_len)) {
+                        if (p.err) atomicOr(p.err, ERR_SEQ);  // more new tokens than positions, or no rotation row
+                    } else {
+                        k.rope = r;
+                        k.row = page_row(p.pages, p.seqs, s, 0, k.pos, p.err);
+                    }
+                }
+            }
+            tok_s[warp] = k;
+        }
+    }
+    __syncthreads();
+    const int hw = threadIdx.x >> 4;
+    const Token k = tok_s[hw % TOK];
+    if (k.rope < 0) return;
+    const int t = blockIdx.x * TOK + hw % TOK, pos = k.pos;
+    const unsigned mask = lane < 16 ? 0x0000ffffu : 0xffff0000u;  // shuffles stay within the half
+    float cs[4], sn[4], w[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 4; ++e) {
         cs[e] = 1.f;
         sn[e] = 0.f;
     }
-    if (live && p.rope != nullptr) {
-        const int r = p.rope_rows != nullptr ? p.rope_rows[t] : pos;
-        if ((unsigned)r >= (unsigned)p.rope_len) {
-            live = false;
-            if (p.err && l == 0) atomicOr(p.err, ERR_SEQ);
-        } else {
-            const float4* c4 = reinterpret_cast<const float4*>(p.rope + (long long)r * 64 + 8 * (l & 7));
+    if (p.rope != nullptr) {
+        const float4* c4 = reinterpret_cast<const float4*>(p.rope + (long long)k.rope * 64 + 4 * l);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float4 c = c4[e];
-                cs[2 * e] = c.x; sn[2 * e] = c.y;
-                cs[2 * e + 1] = c.z; sn[2 * e + 1] = c.w;
+        for (int e = 0; e < 2; ++e) {
+            const float4 c = c4[e];
+            cs[2 * e] = c.x; sn[2 * e] = c.y;
+            cs[2 * e + 1] = c.z; sn[2 * e + 1] = c.w;
+        }
+    }
+    const TI* row = reinterpret_cast<const TI*>(p.qkv) + (long long)t * p.qkv_stride + 4 * l;
+    // Vectors first, first + STEP, .. below end: loads of U at a time, then `finish` for each.
+    auto each = [&](int first, int end, auto&& finish) {
+#pragma unroll 1
+        for (int v0 = first; v0 < end; v0 += U * STEP) {
+            Raw4<TI> raw[U][2];
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+                if (v0 + i * STEP < end) {
+                    raw[i][0].load(row + (v0 + i * STEP) * HD);
+                    raw[i][1].load(row + (v0 + i * STEP) * HD + 64);
+                }
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                if (v0 + i * STEP >= end) break;
+                float x[8];
+                unpack4(raw[i][0], x);
+                unpack4(raw[i][1], x + 4);
+                finish(v0 + i * STEP, x);
             }
         }
-    }
-    if (l < 8) {  // the first half of a pair turns by -sin
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sn[e] = -sn[e];
-    }
-    float x[VPT][8];
-    const TI* row = reinterpret_cast<const TI*>(p.qkv) + (long long)t * p.qkv_stride + 8 * l;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        if (live && v0 + i < n_vec) {
-            load8<TI>(row + (long long)(v0 + i) * HD, x[i]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
-        }
-    }
-    long long crow = -1;  // pool row of kv head 0
-    if (live && v0 + VPT > p.n_q) crow = page_row(p.pages, p.seqs, s, 0, pos, l == 0 ? p.err : nullptr);
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const int vi = v0 + i;
-        const bool is_v = vi >= p.n_q + n_kv, is_q = vi < p.n_q;
-        const float* nw = is_v ? nullptr : is_q ? p.q_norm : p.k_norm;
-        if (nw != nullptr) {
-            float w[8];
-            load8<float>(nw + 8 * l, w);
+    };
+    auto norm_turn = [&](float (&x)[8], bool norm) {
+        if (norm) {
             float ss = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss = fmaf(x[i][e], x[i][e], ss);
-            const unsigned half_mask = lane < 16 ? 0x0000ffffu : 0xffff0000u;
+            for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(half_mask, ss, o);
-            const float r = 1.0f / sqrtf(ss / (float)HD + p.eps);
+            for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+            const float r = rsqrtf(fmaf(ss, 1.f / HD, p.eps));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e] = x[i][e] * r * w[e];
+            for (int e = 0; e < 8; ++e) x[e] = x[e] * r * w[e];
         }
-        __syncwarp();
-        if (p.rope != nullptr) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float other = __shfl_xor_sync(0xffffffffu, x[i][e], 8);
-                if (!is_v) x[i][e] = x[i][e] * cs[e] + other * sn[e];
-            }
+        for (int e = 0; e < 4; ++e) {
+            const float a = x[e], b = x[e + 4];
+            x[e] = a * cs[e] - b * sn[e];
+            x[e + 4] = b * cs[e] + a * sn[e];
         }
-        float amax = 0.f;
-        bool bad = false;
-        if (KVD == KV_Q8) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                amax = fmaxf(amax, fabsf(x[i][e]));
-                bad |= !(fabsf(x[i][e]) <= 3.402823466e38f);
-            }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            const unsigned b = __ballot_sync(0xffffffffu, bad);
-            bad = (lane < 16 ? b & 0xffffu : b >> 16) != 0;
+    };
+    if (p.q_out != nullptr) {
+        const bool norm = p.q_norm != nullptr;
+        if (norm) {
+            load4(p.q_norm + 4 * l, w);
+            load4(p.q_norm + 64 + 4 * l, w + 4);
         }
-        if (!live || vi >= n_vec) continue;
-        if (is_q) {
-            if (p.q_out != nullptr)
-                store8<TQ>(reinterpret_cast<TQ*>(p.q_out) + (long long)t * p.q_stride + vi * HD + 8 * l, x[i]);
-            continue;
-        }
-        if (crow < 0) continue;
-        const int h = is_v ? vi - p.n_q - n_kv : vi - p.n_q;
-        const long long r = crow + h * p.pages.head_rows;
+        TQ* out = reinterpret_cast<TQ*>(p.q_out) + (long long)t * p.q_stride + 4 * l;
+        each(hw / TOK, p.n_q, [&](int v, float (&x)[8]) {
+            norm_turn(x, norm);
+            store4(out + v * HD, x);
+            store4(out + v * HD + 64, x + 4);
+        });
+    }
+    if (k.row < 0) return;
+    const bool norm = p.k_norm != nullptr;
+    if (norm) {
+        load4(p.k_norm + 4 * l, w);
+        load4(p.k_norm + 64 + 4 * l, w + 4);
+    }
+    // places of the lane's two fours in a cached 16-bit row: half of chunk l / 2, and of chunk 8 + l / 2
+    const int at0 = 8 * ((l >> 1) ^ (pos & 7)) + 4 * (l & 1);
+    each(p.n_q + hw / TOK, p.n_q + 2 * n_kv, [&](int v, float (&x)[8]) {
+        const bool is_v = v >= p.n_q + n_kv;
+        const int h = v - p.n_q - (is_v ? n_kv : 0);
+        if (!is_v) norm_turn(x, norm);
+        const long long r = k.row + h * p.pages.head_rows;
         uint8_t* pool = is_v ? p.pages.v : p.pages.k;
         if (KVD == KV_Q8) {
-            float sc = amax / 127.0f;
-            if (sc == 0.f) sc = 1.f;
-            uint32_t c[2] = {0u, 0u};
-            if (!bad) {
+            float amax = 0.f;  // (NaN when the row holds one)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int q = max(-127, min(127, __float2int_rn(x[i][e] / sc)));
-                    c[e >> 2] |= (uint32_t)(q & 0xff) << (8 * (e & 3));
-                }
+            for (int e = 0; e < 8; ++e) amax = max_nan(amax, fabsf(x[e]));
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(mask, amax, o));
+            float sc = amax * (1.f / 127.f);
+            if (sc == 0.f) sc = 1.f;
+            uint32_t c[8];
+            if (sc > 1e-30f) {  // x times the reciprocal is within 2^-15 of a step; 1.5 x 2^23 rounds it into the low byte
+                const float inv = __fdividef(1.0f, sc);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) c[e] = __float_as_uint(fmaf(x[e], inv, 12582912.f));
+            } else {  // (the reciprocal may pass fp32's range)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) c[e] = (uint32_t)max(-127, min(127, __float2int_rn(x[e] / sc)));
             }
-            *reinterpret_cast<uint2*>(pool + r * HD + 8 * l) = make_uint2(c[0], c[1]);
+            const bool bad = !(amax <= 3.402823466e38f);
+            uint8_t* o = pool + r * HD + 4 * l;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                *reinterpret_cast<uint32_t*>(o + 64 * e) =
+                    bad ? 0u : __byte_perm(__byte_perm(c[4 * e], c[4 * e + 1], 0x0040), __byte_perm(c[4 * e + 2], c[4 * e + 3], 0x0040), 0x5410);
             if (l == 0) (is_v ? p.pages.vs : p.pages.ks)[r] = bad ? __int_as_float(0x7fc00000) : sc;
         } else {
-            store8<TC>(reinterpret_cast<TC*>(pool) + r * HD + 8 * (l ^ (pos & 7)), x[i]);
+            TC* o = reinterpret_cast<TC*>(pool) + r * HD + at0;
+            store4(o, x);
+            store4(o + 64, x + 4);
         }
-    }
+    });
 }
 
 struct KvReadParams {

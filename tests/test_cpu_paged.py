@@ -33,7 +33,8 @@ BAD_PAGES = [dict(k=None), dict(v=None), dict(k=A + 8), dict(v=A + 4), dict(dtyp
              dict(page_size=0), dict(page_size=8), dict(page_size=48), dict(page_size=512), dict(n_pages=-1),
              dict(dtype=L.KV_Q8), dict(dtype=L.KV_Q8, k_scale=A), dict(dtype=L.KV_Q8, k_scale=A, v_scale=A + 4),
              dict(page_rows=32), dict(head_rows=16), dict(page_rows=16, head_rows=8), dict(page_rows=-32, head_rows=16),
-             dict(page_rows=24, head_rows=16), dict(page_rows=32, head_rows=24)]
+             dict(page_rows=24, head_rows=16), dict(page_rows=32, head_rows=24),
+             dict(n_pages=2**31 - 1), dict(page_rows=2**60, head_rows=16), dict(page_rows=32, head_rows=2**62)]
 BAD_SEQS = [dict(n_seqs=-1), dict(n_seqs=1025), dict(total_q=-1), dict(max_q=-1), dict(max_kv=-1), dict(max_pages=-1), dict(cu_q=None),
             dict(kv_len=None), dict(page_table=None), dict(cu_q=A + 2), dict(page_table=A + 1), dict(max_pages=1 << 28)]
 BAD_ROWS = [dict(qkv=None), dict(qkv=A + 4), dict(qkv_dtype=3), dict(qkv_dtype=-1), dict(n_q=-1), dict(n_q=257), dict(q_dtype=L.DT_F32),
@@ -89,7 +90,6 @@ def test_null_descriptors_outputs_and_flags():
     refused(lib.icua_attn_paged(p, s, None, None, None))
     refused(lib.icua_attn_paged(p, s, C.byref(attn()), A + 1, None))
     big = seqs(total_q=2**31 - 1)
-    refused(lib.icua_kv_write(p, C.byref(big), C.byref(rows(n_q=256)), None, None))
     refused(lib.icua_attn_paged(p, C.byref(big), C.byref(attn()), None, None))
 
 
