@@ -159,8 +159,8 @@ cudaError_t launch_attn(const PagedAttnParams& p, int dev, cudaStream_t st) {
     const int smem = pa_smem(Q8, MT, 1);
     cudaError_t e = allow_smem<paged_attn_kernel<T, Q8, MT, 1>>(smem, dev);
     if (e != cudaSuccess) return e;
-    const int ctas = std::min(PA_MAX_CTAS, pa_ctas(Q8, MT) * sm_count(dev));
-    paged_attn_kernel<T, Q8, MT, 1><<<ctas, PA_THREADS, smem, st>>>(p);
+    const int ctas = std::min(PA_MAX_CTAS, pa_ctas(Q8, MT, 1) * sm_count(dev));
+    paged_attn_kernel<T, Q8, MT, 1><<<ctas, 32 * pa_warps(1), smem, st>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
@@ -182,7 +182,7 @@ cudaError_t launch_attn_cluster(const PagedAttnParams& p, int dev, cudaStream_t 
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.seqs.n_seqs * p.pages.n_kv * PA_CLUSTER);
-    cfg.blockDim = dim3(PA_THREADS);
+    cfg.blockDim = dim3(32 * pa_warps(PA_CLUSTER));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at[1];
@@ -209,7 +209,7 @@ cudaError_t launch_attn_rows(const PagedAttnParams& p, bool f16, bool q8, bool c
 
 // Sequences with up to PA_ROWS_FEW query rows per kv head go through the warp-MMA kernel, more rows
 // through the tensor-core kernel.
-constexpr int PA_ROWS_FEW = 64;
+constexpr int PA_ROWS_FEW = 32;
 constexpr int PA_CLUSTER_KEYS = 4096;
 
 // Tiles of the tensor-core kernel: a bound from what the host knows, and the shares of the keys that fill
@@ -395,7 +395,7 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
         // Few items, up to PA_CLUSTER_KEYS keys each: a cluster per item does without the second launch.  Longer
         // ones want every SM, and more of them fill the GPU by themselves.
         const bool cluster = one_tile && seqs->max_kv <= PA_CLUSTER_KEYS &&
-                             (int64_t)seqs->n_seqs * pages->n_kv * PA_CLUSTER <= 2 * sm_count(dev);
+                             (int64_t)seqs->n_seqs * pages->n_kv * PA_CLUSTER <= sm_count(dev);
         if (cluster) p.max_rows = 16;
         e = one_tile ? launch_attn_rows<1>(p, f16, q8, cluster, dev, s) : launch_attn_rows<2>(p, f16, q8, false, dev, s);
     }

@@ -31,9 +31,8 @@
 namespace icua {
 
 constexpr int PA_ROWS_MAX = 32;   // query rows per item: 16 or 32
-constexpr int PA_WARPS = 4;
-constexpr int PA_THREADS = PA_WARPS * 32;
-constexpr int PA_ITEM = 2;
+constexpr int pa_warps(int cl) { return cl > 1 ? 8 : 4; }  // (a cluster's CTAs have their SM to themselves)
+constexpr int PA_ITEM = 3;
 constexpr int PA_CLUSTER = 8;     // CTAs that share an item in the small-batch form
 constexpr int PA_MAX_CTAS = 480;  // workspace slots are laid out for so many
 constexpr int PA_MAX_SEQS = 1024;
@@ -62,16 +61,16 @@ struct PagedAttnParams {
 };
 
 constexpr int pa_keys(bool q8) { return q8 ? 32 : 16; }  // rows of a warp's slot
-constexpr int pa_block(bool q8) { return PA_WARPS * pa_keys(q8); }
+constexpr int pa_block(bool q8, int cl) { return pa_warps(cl) * pa_keys(q8); }
 constexpr int pa_slot(bool q8) { return q8 ? 32 * 2 * HD + 2 * 32 * 4 : 16 * 2 * HD * 2; }
 // CTAs per SM and ring slots per warp.  Sixteen rows of a q8 cache: three CTAs (their fragments' conversion is
 // a chain of dependent instructions, which more warps hide), with the q fragments in shared memory to fit the
 // registers.  Else two, which stream a 16-bit cache at HBM speed.
-constexpr int pa_ctas(bool q8, int mt) { return q8 && mt == 1 ? 3 : 2; }
-constexpr int pa_ns(bool q8, int mt) { return pa_ctas(q8, mt) == 3 ? 2 : 3; }
+constexpr int pa_ctas(bool q8, int mt, int cl) { return cl > 1 ? 1 : q8 && mt == 1 ? 3 : 2; }
+constexpr int pa_ns(bool q8, int mt, int cl) { return pa_ctas(q8, mt, cl) == 2 ? 3 : 2; }
 constexpr bool pa_q_in_smem(bool q8, int mt) { return mt > 1 || q8; }
 constexpr int pa_smem(bool q8, int mt, int cl) {
-    return PA_WARPS * pa_ns(q8, mt) * pa_slot(q8) + (pa_q_in_smem(q8, mt) ? mt * 16 * 2 * HD : 0) + (cl > 1 ? 0 : (PA_MAX_SEQS + 1) * 4);
+    return pa_warps(cl) * pa_ns(q8, mt, cl) * pa_slot(q8) + (pa_q_in_smem(q8, mt) ? mt * 16 * 2 * HD : 0) + (cl > 1 ? 0 : (PA_MAX_SEQS + 1) * 4);
 }
 
 __device__ __forceinline__ void cluster_barrier() {
@@ -219,10 +218,10 @@ struct PaDeal {
 // head) of the cluster's number, and join its parts through distributed shared memory.  One launch and no
 // workspace, for calls whose time is latency.
 template <typename T, bool Q8, int MT, int CL>
-__global__ void __launch_bounds__(PA_THREADS, pa_ctas(Q8, MT)) paged_attn_kernel(const PagedAttnParams p) {
-    constexpr int PA_NS = pa_ns(Q8, MT);
+__global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_attn_kernel(const PagedAttnParams p) {
+    constexpr int PA_WARPS = pa_warps(CL), PA_THREADS = 32 * PA_WARPS, PA_NS = pa_ns(Q8, MT, CL);
     constexpr bool QS = pa_q_in_smem(Q8, MT);
-    constexpr int KEYS = pa_keys(Q8), BLOCK = pa_block(Q8), SLOT = pa_slot(Q8), NT = KEYS / 8, ROWS = 16 * MT;
+    constexpr int KEYS = pa_keys(Q8), BLOCK = pa_block(Q8, CL), SLOT = pa_slot(Q8), NT = KEYS / 8, ROWS = 16 * MT;
     constexpr int ROW = Q8 ? HD : 2 * HD;  // bytes of a cached row
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float ml[PA_WARPS][2][ROWS];
@@ -673,7 +672,8 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas(Q8, MT)) paged_attn_kernel
                 }
             }
             __syncthreads();
-            const int r = tid >> 3, rt = 16 * mt + r;  // eight threads a row, sixteen columns each
+            constexpr int TPR = PA_THREADS / 16;  // threads a row, chunks of eight columns in turn
+            const int r = tid / TPR, rt = 16 * mt + r;
             const int rr = tile * ROWS + rt;
             if (rr < rows) {
                 float mm = ml[0][0][rt];
@@ -688,8 +688,8 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas(Q8, MT)) paged_attn_kernel
                 const float il = mm == -INFINITY ? 0.f : 1.0f / ll;
                 T* dst = reinterpret_cast<T*>(p.out) + (c.w.q0 + rr / G) * p.out_stride + (h * G + rr % G) * HD;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int col = 8 * ((tid & 7) + 8 * i);
+                for (int i = 0; i < 16 / TPR; ++i) {
+                    const int col = 8 * (tid % TPR + TPR * i);
                     float y[8];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
@@ -717,11 +717,11 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas(Q8, MT)) paged_attn_kernel
                         store8<float>(pt + rt * HD + col, y);
                     }
                 }
-                if (CL > 1 && (tid & 7) == 0) {
+                if (CL > 1 && tid % TPR == 0) {
                     ml_c[0][rt] = mm;
                     ml_c[1][rt] = ll;
                 }
-                if (CL == 1 && !whole && (tid & 7) == 0) {
+                if (CL == 1 && !whole && tid % TPR == 0) {
                     pt[PA_ROWS_MAX * HD + rt] = mm;
                     pt[PA_ROWS_MAX * HD + PA_ROWS_MAX + rt] = ll;
                 }
@@ -732,7 +732,7 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas(Q8, MT)) paged_attn_kernel
             cluster_barrier();
             const int r = tid >> 3, rr = tile * ROWS + r, rank = blockIdx.x % CL;
             const int col = (HD / CL) * rank + 2 * (tid & 7);
-            if (rr < rows) {
+            if (tid < 128 && rr < rows) {
                 float pm[CL], pl[CL], px[CL], py[CL];
 #pragma unroll
                 for (int k = 0; k < CL; ++k) {
