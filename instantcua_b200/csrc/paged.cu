@@ -234,7 +234,7 @@ cudaError_t launch_attn_tc(const PagedTcParams& p, int tiles, int dev, cudaStrea
     paged_attn_tc_kernel<T, Q8><<<tiles * p.pages.n_kv * p.n_split, PC_THREADS, PcSmem<Q8>::alloc, st>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess || p.n_split == 1) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tiles * p.pages.n_kv * 32);
+    cfg.gridDim = dim3(tiles * p.pages.n_kv * 8);
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute at[1];

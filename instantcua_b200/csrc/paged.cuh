@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(256, sizeof(TI) == 4 ? 3 : 4) kv_write_kernel(
     };
     __shared__ Token tok_s[TOK];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & 15;
-    const int n_kv = p.pages.n_kv, n_vec = p.n_q + 2 * n_kv;
+    const int n_kv = p.pages.n_kv;
     if (warp < TOK) {
         const int t = blockIdx.x * TOK + warp;
         const int s = t < p.seqs.total_q ? find_seq(p.seqs, t, lane) : p.seqs.n_seqs;

@@ -248,6 +248,9 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
             tile_s = t;
             live_s = live;
         }
+    } else if (warp == 8) {
+        tmem_alloc(&tmem_slot, PC_TMEM_COLS);
+        tmem_relinquish();
     } else if (threadIdx.x == 32) {
         mbar_init(q_full, 128);
         for (int i = 0; i < 2; ++i) {
@@ -264,17 +267,15 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
         mbar_init(done, 1);
         fence_mbar_init();
     }
-    __syncthreads();
-    pdl_launch_dependents();
-    if (!live_s) return;
-    if (warp == 8) {
-        tmem_alloc(&tmem_slot, PC_TMEM_COLS);
-        tmem_relinquish();
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();
     const uint32_t tmem = tmem_slot;
+    if (!live_s) {
+        if (warp == 8) tmem_dealloc(tmem, PC_TMEM_COLS);
+        return;
+    }
     const PcTile t = tile_s;
     const int rows = t.n * G, nblk = t.j1 - t.j0;
     // blocks of the half: its last row sees no further
@@ -290,6 +291,24 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
         // ---- producers -----------------------------------------------------------------------------
         const int w = warp - 12;
         bool ok = true;
+        // This warp's keys 32 w .. 32 w + 31 of a block lie in two pages at most, sixteen each.  The table is
+        // read one block ahead (raw entries; -2: past the sequence's end).
+        const int* table = p.seqs.table + (long long)t.s * p.seqs.max_pages;
+        auto entry = [&](int j, int part) -> int {
+            const int pos = j * PC_BK + 32 * w + 16 * part;
+            return j < t.j1 && pos < t.kv ? table[pos >> ps_shift] : -2;
+        };
+        // pool row of the first of the sixteen keys (all ones: none of them is to be read)
+        auto row_of = [&](int page, int j, int part) -> uint32_t {
+            if ((unsigned)page >= (unsigned)p.pages.n_pages) {
+                if (page != -2 && lane == 0 && p.err) atomicOr(p.err, ERR_PAGE);
+                return 0xffffffffu;
+            }
+            const int pos = j * PC_BK + 32 * w + 16 * part;
+            return (uint32_t)(page * p.pages.page_rows + h * p.pages.head_rows + (pos & ((1 << ps_shift) - 1)));
+        };
+        int ahead[2] = {entry(t.j0, 0), entry(t.j0, 1)};
+        // the q rows first; they are announced like the copies that follow them
         {
             const T* qrow[2];
             bool real[2];
@@ -314,27 +333,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
                                reinterpret_cast<const uint8_t*>(a) + c * 16, rl);
                 }
             cp_async_commit();
-            cp_async_wait<0>();
-            fence_proxy_async_smem();
-            mbar_arrive(q_full);
         }
-        // This warp's keys 32 w .. 32 w + 31 of a block lie in two pages at most, sixteen each.  The table is
-        // read one block ahead (raw entries; -2: past the sequence's end).
-        const int* table = p.seqs.table + (long long)t.s * p.seqs.max_pages;
-        auto entry = [&](int j, int part) -> int {
-            const int pos = j * PC_BK + 32 * w + 16 * part;
-            return j < t.j1 && pos < t.kv ? table[pos >> ps_shift] : -2;
-        };
-        // pool row of the first of the sixteen keys (all ones: none of them is to be read)
-        auto row_of = [&](int page, int j, int part) -> uint32_t {
-            if ((unsigned)page >= (unsigned)p.pages.n_pages) {
-                if (page != -2 && lane == 0 && p.err) atomicOr(p.err, ERR_PAGE);
-                return 0xffffffffu;
-            }
-            const int pos = j * PC_BK + 32 * w + 16 * part;
-            return (uint32_t)(page * p.pages.page_rows + h * p.pages.head_rows + (pos & ((1 << ps_shift) - 1)));
-        };
-        int ahead[2] = {entry(t.j0, 0), entry(t.j0, 1)};
         if (!Q8) {
             const int c = lane & 15;
             // rows 2 k + lane / 16 of each sixteen; `left`: the sequence's keys from the first one on
@@ -353,12 +352,18 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
             // Copies are announced two items behind, three in flight, so that their latency is covered; a
             // producer that has to wait for room announces everything first.
             PcRing<NS> put, tell;
-            int untold = 0;
+            int untold = 1;
+            bool q_told = false;
             auto tell_one = [&]() {
                 fence_proxy_async_smem();
+                --untold;
+                if (!q_told) {
+                    q_told = true;
+                    mbar_arrive(q_full);
+                    return;
+                }
                 mbar_arrive(&kv_full[tell.slot]);
                 tell.next();
-                --untold;
             };
             for (int i = 0; ok && i < nblk; ++i) {
                 const int j = t.j0 + i;
@@ -428,6 +433,9 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
             };
             uint32_t row[2] = {row_of(ahead[0], t.j0, 0), row_of(ahead[1], t.j0, 1)};
             if (nblk > 0) load(rk, p.pages.k, row, t.kv - t.j0 * PC_BK - 32 * w);
+            cp_async_wait<0>();
+            fence_proxy_async_smem();
+            mbar_arrive(q_full);
             for (int i = 0; i < nblk; ++i) {
                 const int j = t.j0 + i, left = t.kv - j * PC_BK - 32 * w;
                 ahead[0] = entry(j + 1, 0);
@@ -636,30 +644,50 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
         if (!ok) {
             if (lane == 0 && p.err) atomicOr(p.err, ERR_WAIT_PREFILL);
         } else {
-            const bool real = R < rows;
-            const float il = p.n_split > 1 ? 1.f : m == -INFINITY ? 0.f : 1.0f / (l.x + l.y);
-            const int Rc = min(R, rows - 1);
-            T* dst = reinterpret_cast<T*>(p.out) + (t.q0 + Rc / G) * p.out_stride + (h * G + Rc % G) * HD;
-            float* pt = p.part + (size_t)blockIdx.x * PC_PART;
-            const int rt = 128 * hf + 32 * quarter + lane;
+            const float sum = l.x + l.y;
+            const int rt = 128 * hf + 32 * quarter + lane;  // row of the tile
+            if (p.n_split > 1) {  // parts lie [32 chunks of four columns][256 rows]: the warp's stores are contiguous
+                float* pt = p.part + (size_t)blockIdx.x * PC_PART;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                float v[32];
-                if (nb > 0) tmem_ld32(o_tm + 32 * c, v);
+                for (int c = 0; c < 4; ++c) {
+                    float v[32];
+                    if (nb > 0) tmem_ld32(o_tm + 32 * c, v);
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    float x[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = nb > 0 && il != 0.f ? v[8 * b + e] * il : 0.f;
-                    if (real) {
-                        if (p.n_split > 1) store8<float>(pt + rt * HD + 32 * c + 8 * b, x);
-                        else store8<T>(dst + 32 * c + 8 * b, x);
+                    for (int b = 0; b < 8; ++b) {
+                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (nb > 0) x = make_float4(v[4 * b], v[4 * b + 1], v[4 * b + 2], v[4 * b + 3]);
+                        *reinterpret_cast<float4*>(pt + ((8 * c + b) * PC_ROWS + rt) * 4) = x;
                     }
                 }
-            }
-            if (p.n_split > 1) {
                 pt[PC_ROWS * HD + rt] = m;
-                pt[PC_ROWS * HD + PC_ROWS + rt] = l.x + l.y;
+                pt[PC_ROWS * HD + PC_ROWS + rt] = sum;
+            } else {
+                // through the half's q tile, which no product reads any more (16-byte chunk c of row r at c ^ (r & 15)),
+                // so that the warp writes whole rows
+                const float il = nb == 0 || m == -INFINITY ? 0.f : 1.0f / sum;
+                uint8_t* o_s = smem + S::q_off + rt * 256;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float v[32];
+                    if (nb > 0) tmem_ld32(o_tm + 32 * c, v);
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        float x[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = il != 0.f ? v[8 * b + e] * il : 0.f;
+                        store8<T>(reinterpret_cast<T*>(o_s + (((4 * c + b) ^ (rt & 15)) << 4)), x);
+                    }
+                }
+                __syncwarp();
+                const int ch = lane & 15;
+#pragma unroll 4
+                for (int k = 0; k < 16; ++k) {
+                    const int r = 128 * hf + 32 * quarter + 2 * k + (lane >> 4), rr = t.row0 + r;
+                    if (rr < rows)
+                        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + (t.q0 + rr / G) * p.out_stride + (h * G + rr % G) * HD +
+                                                  8 * ch) =
+                            *reinterpret_cast<const uint4*>(smem + S::q_off + r * 256 + ((ch ^ (r & 15)) << 4));
+                }
             }
         }
     }
@@ -672,36 +700,55 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
     }
 }
 
-// Folds the n_split parts of every row, in the order of the keys.  Grid: n_kv x tiles x 32, eight rows a CTA.
+// Folds the n_split parts of every row, in the order of the keys.  Grid: n_kv x tiles x 8; a CTA takes 32 rows, lane
+// = row and warp = four chunks of four columns (as the parts lie), and turns them in shared memory to write rows.
 template <typename T>
 __global__ void __launch_bounds__(256) paged_attn_tc_join_kernel(const PagedTcParams p) {
+    __shared__ __align__(16) uint2 o_s[32][33];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n_kv = p.pages.n_kv, G = p.group;
-    const int rt = (blockIdx.x & 31) * 8 + warp, h = (blockIdx.x >> 5) % n_kv, y = (blockIdx.x >> 5) / n_kv;
+    const int r0 = (blockIdx.x & 7) * 32, h = (blockIdx.x >> 3) % n_kv, y = (blockIdx.x >> 3) / n_kv;
     PcTile t{};
     const bool live = pc_find(p.seqs, p.pages.ps_shift, G, p.min_rows, y, lane, t, nullptr);
+    if (!live || t.row0 + r0 >= t.n * G) return;
     pdl_wait();
-    const int R = t.row0 + rt;
-    if (!live || R >= t.n * G) return;
+    const float* pt0 = p.part + (size_t)(h + n_kv * p.n_split * y) * PC_PART + r0 + lane;
     float m = -INFINITY, l = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+    float4 a[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) a[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
     for (int z = 0; z < p.n_split; ++z) {
-        const float* pt = p.part + (size_t)(h + n_kv * (z + p.n_split * y)) * PC_PART;
-        const float pm = pt[PC_ROWS * HD + rt], pl = pt[PC_ROWS * HD + PC_ROWS + rt];
-        const float4 v = *reinterpret_cast<const float4*>(pt + rt * HD + 4 * lane);
+        const float* pt = pt0 + (size_t)n_kv * z * PC_PART;
+        const float pm = pt[PC_ROWS * HD], pl = pt[PC_ROWS * HD + PC_ROWS];
+        float4 v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            v[c] = *reinterpret_cast<const float4*>(pt - r0 - lane + ((4 * warp + c) * PC_ROWS + r0 + lane) * 4);
         const float mn = fmaxf(m, pm);
-        const float f0 = m == -INFINITY ? 0.f : exp2f(m - mn), f1 = pm == -INFINITY ? 0.f : exp2f(pm - mn);
+        const float f0 = m == -INFINITY ? 0.f : ex2_approx(m - mn), f1 = pm == -INFINITY ? 0.f : ex2_approx(pm - mn);
         m = mn;
         l = l * f0 + pl * f1;
-        a.x = a.x * f0 + v.x * f1;
-        a.y = a.y * f0 + v.y * f1;
-        a.z = a.z * f0 + v.z * f1;
-        a.w = a.w * f0 + v.w * f1;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            a[c].x = a[c].x * f0 + v[c].x * f1;
+            a[c].y = a[c].y * f0 + v[c].y * f1;
+            a[c].z = a[c].z * f0 + v[c].z * f1;
+            a[c].w = a[c].w * f0 + v[c].w * f1;
+        }
     }
     const float il = m == -INFINITY ? 0.f : 1.0f / l;
-    T* dst = reinterpret_cast<T*>(p.out) + (t.q0 + R / G) * p.out_stride + (h * G + R % G) * HD + 4 * lane;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_f<T>(a.x * il, a.y * il), pack_f<T>(a.z * il, a.w * il));
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        o_s[lane][4 * warp + c] = make_uint2(pack_f<T>(a[c].x * il, a[c].y * il), pack_f<T>(a[c].z * il, a[c].w * il));
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int r = 4 * warp + k, R = t.row0 + r0 + r;
+        if (R < t.n * G)
+            *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + (t.q0 + R / G) * p.out_stride + (h * G + R % G) * HD + 4 * lane) =
+                o_s[r][lane];
+    }
 }
 
 }  // namespace icua
