@@ -349,7 +349,7 @@ typedef struct icua_kv_pages {
     int32_t dtype;      /* ICUA_KV_F16, ICUA_KV_BF16 or ICUA_KV_Q8 */
     int32_t n_kv;       /* kv heads, 1..128 */
     int32_t page_size;  /* positions per page: 16, 32, 64, 128 or 256 */
-    int32_t n_pages;
+    int32_t n_pages;    /* at least 1 */
     int64_t page_rows, head_rows;
 } icua_kv_pages;
 
@@ -365,7 +365,7 @@ typedef struct icua_kv_seqs {
     const int32_t* cu_q;       /* [n_seqs + 1], ascending */
     const int32_t* kv_len;     /* [n_seqs] */
     const int32_t* page_table; /* [n_seqs][max_pages]: entries up to a sequence's last page are read */
-    int32_t max_pages;
+    int32_t max_pages;         /* max_pages * page_size: at most 2^30 */
 } icua_kv_seqs;
 
 /* New tokens on their way into the cache: rows q | k | v of (n_q + 2 n_kv) * 128 elements. */

@@ -56,7 +56,7 @@ icua_status check_cache(const icua_kv_pages* c, const icua_kv_seqs* s, PagesView
     int sh = 4;
     while (sh < 8 && (1 << sh) != c->page_size) ++sh;
     if ((1 << sh) != c->page_size) return bad("page_size %d is not 16, 32, 64, 128 or 256", c->page_size);
-    if (c->n_pages < 0) return bad("n_pages is negative");
+    if (c->n_pages < 1) return bad("n_pages is below 1");
     if (!c->k || !c->v || !aligned(c->k, 16) || !aligned(c->v, 16)) return bad("pools are null or not 16-byte aligned");
     if (c->dtype == ICUA_KV_Q8 && (!c->k_scale || !c->v_scale || !aligned(c->k_scale, 16) || !aligned(c->v_scale, 16)))
         return bad("scales of a q8 cache are null or not 16-byte aligned");
@@ -74,7 +74,7 @@ icua_status check_cache(const icua_kv_pages* c, const icua_kv_seqs* s, PagesView
         return bad("the pool is too large");
     if (s->n_seqs > 0 && (!s->cu_q || !s->kv_len || (s->max_pages > 0 && !s->page_table))) return bad("null batch arrays");
     if (!aligned(s->cu_q, 4) || !aligned(s->kv_len, 4) || !aligned(s->page_table, 4)) return bad("batch arrays are not aligned");
-    if ((int64_t)s->max_pages * c->page_size > INT32_MAX) return bad("max_pages * page_size is above 2^31 - 1");
+    if ((int64_t)s->max_pages * c->page_size > 1 << 30) return bad("max_pages * page_size is above 2^30");
     P->k = (uint8_t*)c->k;
     P->v = (uint8_t*)c->v;
     P->ks = c->k_scale;
@@ -254,7 +254,7 @@ icua_status check_attn(const icua_kv_pages* pages, const icua_kv_seqs* seqs, int
     if (n_q < pages->n_kv || n_q > 256 || n_q % pages->n_kv) return bad("n_q %d is not a multiple of n_kv %d up to 256", n_q, pages->n_kv);
     // the kernels count blocks of keys over all items in 32 bits
     const int64_t rows = (int64_t)seqs->total_q * (n_q / pages->n_kv);
-    const double blocks = ((double)rows / 16 + seqs->n_seqs) * pages->n_kv * ((double)seqs->max_pages * pages->page_size / 64 + 1);
+    const double blocks = ((double)rows / 16 + seqs->n_seqs) * pages->n_kv * ((double)seqs->max_pages * pages->page_size / 64 + 1 + PA_ITEM);
     if (rows > INT32_MAX || blocks > 4e9) return bad("the batch is too large: split it");
     return ICUA_OK;
 }

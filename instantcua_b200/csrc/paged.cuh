@@ -69,6 +69,18 @@ __device__ __forceinline__ int find_seq(const SeqsView& S, int t, int lane) {
     return c;
 }
 
+// Maxima that keep a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 struct KvWriteParams {
     PagesView pages;
     SeqsView seqs;
@@ -172,12 +184,6 @@ template <typename T>
 __device__ __forceinline__ void store4(T* p, const float* x) {
     *reinterpret_cast<uint2*>(p) = make_uint2(pack_f<T>(x[0], x[1]), pack_f<T>(x[2], x[3]));
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-
 // A half-warp per head vector: lane l holds elements 4 l .. 4 l + 3 and 64 + 4 l .., the two halves of four
 // rotation pairs.  y = x rsqrt(mean x^2 + eps) w, then (y_j c - y_{j+64} s, y_{j+64} c + y_j s), in fp32; q rows
 // are rounded to the output type, k and v rows to the cache type or to int8 codes: scale = max|x| / 127 in fp32

@@ -552,25 +552,27 @@ __global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        bm[mt][i] = fmaxf(s[mt][0][2 * i], s[mt][0][2 * i + 1]);
+                        // (a NaN among the scores becomes the maximum, and the row's result)
+                        bm[mt][i] = max_nan(s[mt][0][2 * i], s[mt][0][2 * i + 1]);
 #pragma unroll
-                        for (int nt = 1; nt < NT; ++nt) bm[mt][i] = fmaxf(bm[mt][i], fmaxf(s[mt][nt][2 * i], s[mt][nt][2 * i + 1]));
+                        for (int nt = 1; nt < NT; ++nt) bm[mt][i] = max_nan(bm[mt][i], s[mt][nt][2 * i], s[mt][nt][2 * i + 1]);
                     }
 #pragma unroll
                 for (int x = 1; x < 4; x <<= 1)
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) bm[mt][i] = fmaxf(bm[mt][i], __shfl_xor_sync(0xffffffffu, bm[mt][i], x));
-                bool move = false;
+                        for (int i = 0; i < 2; ++i) bm[mt][i] = max_nan(bm[mt][i], __shfl_xor_sync(0xffffffffu, bm[mt][i], x));
+                auto moves = [&](int mt, int i) { return !(bm[mt][i] <= m[mt][i] + 8.f) && bm[mt][i] != -INFINITY; };
+                bool any = false;
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) move |= bm[mt][0] > m[mt][0] + 8.f || bm[mt][1] > m[mt][1] + 8.f;
-                if (__any_sync(0xffffffffu, move)) {
+                for (int mt = 0; mt < MT; ++mt) any |= moves(mt, 0) || moves(mt, 1);
+                if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const float mn = bm[mt][i] > m[mt][i] + 8.f ? bm[mt][i] : m[mt][i];
+                            const float mn = moves(mt, i) ? bm[mt][i] : m[mt][i];
                             const float corr = m[mt][i] == -INFINITY ? 0.f : ex2_approx(m[mt][i] - mn);
                             m[mt][i] = mn;
                             l[mt][i] *= corr;
@@ -678,7 +680,7 @@ __global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_
             if (rr < rows) {
                 float mm = ml[0][0][rt];
 #pragma unroll
-                for (int w = 1; w < PA_WARPS; ++w) mm = fmaxf(mm, ml[w][0][rt]);
+                for (int w = 1; w < PA_WARPS; ++w) mm = max_nan(mm, ml[w][0][rt]);
                 float fw[PA_WARPS], ll = 0.f;
 #pragma unroll
                 for (int w = 0; w < PA_WARPS; ++w) {
@@ -747,7 +749,7 @@ __global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_
                 }
                 float mm = pm[0];
 #pragma unroll
-                for (int k = 1; k < CL; ++k) mm = fmaxf(mm, pm[k]);
+                for (int k = 1; k < CL; ++k) mm = max_nan(mm, pm[k]);
                 float ll = 0.f, ax = 0.f, ay = 0.f;
 #pragma unroll
                 for (int k = 0; k < CL; ++k) {
@@ -810,7 +812,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_attn_join_kernel(const Pa
                 }
                 float mn = m;
 #pragma unroll
-                for (int u = 0; u < 8; ++u) mn = fmaxf(mn, pm[u]);
+                for (int u = 0; u < 8; ++u) mn = max_nan(mn, pm[u]);
                 const float f0 = m == -INFINITY ? 0.f : ex2_approx(m - mn);
                 m = mn;
                 l *= f0;
@@ -839,7 +841,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_attn_join_kernel(const Pa
                     const int o = (k << log_r) + warp;
                     const float pm = ml_s[o][0];
                     if (pm == -INFINITY) continue;
-                    const float mn = fmaxf(m, pm), f0 = m == -INFINITY ? 0.f : ex2_approx(m - mn), f1 = ex2_approx(pm - mn);
+                    const float mn = max_nan(m, pm), f0 = m == -INFINITY ? 0.f : ex2_approx(m - mn), f1 = ex2_approx(pm - mn);
                     const float4 v = acc_s[o][lane];
                     m = mn;
                     l = l * f0 + ml_s[o][1] * f1;

@@ -553,7 +553,16 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
         float m = -INFINITY;
         float2 l = make_float2(0.f, 0.f);  // sums of the even and of the odd keys
         bool ok = true;
+        // whether lanes 0-7's sixteen keys of block i lie in a page that does not exist (read a block ahead)
+        const int* table = p.seqs.table + (long long)t.s * p.seqs.max_pages;
+        auto entry = [&](int i) {
+            const int pos = (t.j0 + i) * PC_BK + 16 * lane;
+            return i < nb && lane < 8 && pos < t.kv ? table[pos >> ps_shift] : 0;
+        };
+        int ahead = entry(0);
         for (int i = 0; i < nb; ++i) {
+            const uint32_t gone = __ballot_sync(0xffffffffu, (unsigned)ahead >= (unsigned)p.pages.n_pages);
+            ahead = entry(i + 1);
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(&s_full[hf], i & 1))) {
                 ok = false;
                 break;
@@ -581,21 +590,21 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
                     v[4 * c] = x.x; v[4 * c + 1] = x.y; v[4 * c + 2] = y.x; v[4 * c + 3] = y.y;
                 }
             }
-            if (edge) {
+            if (edge || gone) {
 #pragma unroll
                 for (int c = 0; c < 128; ++c)
-                    if (k0 + c > lim) v[c] = -INFINITY;
+                    if (k0 + c > lim || (gone >> (c >> 4)) & 1u) v[c] = -INFINITY;
             }
-            float bm4[4];
+            float bm4[4];  // (a NaN among the scores becomes the maximum, and the row's result)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                bm4[c] = fmaxf(v[c], v[c + 4]);
+                bm4[c] = max_nan(v[c], v[c + 4]);
 #pragma unroll
-                for (int e = 8; e < 128; e += 8) bm4[c] = fmaxf(bm4[c], fmaxf(v[e + c], v[e + c + 4]));
+                for (int e = 8; e < 128; e += 8) bm4[c] = max_nan(bm4[c], v[e + c], v[e + c + 4]);
             }
             const float sl = Q8 ? 1.f : p.scale_log2;
-            const float bm = fmaxf(fmaxf(bm4[0], bm4[1]), fmaxf(bm4[2], bm4[3])) * sl;
-            const bool move = bm > m + 8.f;  // (from -inf: any finite score)
+            const float bm = max_nan(max_nan(bm4[0], bm4[1]), bm4[2], bm4[3]) * sl;
+            const bool move = !(bm <= m + 8.f) && bm != -INFINITY;  // (from -inf: any score that is seen)
             if (__any_sync(0xffffffffu, move)) {
                 const float corr = move ? (m == -INFINITY ? 0.f : ex2_approx(m - bm)) : 1.f;
                 if (move) m = bm;
@@ -725,7 +734,7 @@ __global__ void __launch_bounds__(256) paged_attn_tc_join_kernel(const PagedTcPa
 #pragma unroll
         for (int c = 0; c < 4; ++c)
             v[c] = *reinterpret_cast<const float4*>(pt - r0 - lane + ((4 * warp + c) * PC_ROWS + r0 + lane) * 4);
-        const float mn = fmaxf(m, pm);
+        const float mn = max_nan(m, pm);
         const float f0 = m == -INFINITY ? 0.f : ex2_approx(m - mn), f1 = pm == -INFINITY ? 0.f : ex2_approx(pm - mn);
         m = mn;
         l = l * f0 + pl * f1;

@@ -30,7 +30,7 @@ def attn(**kw):
 
 
 BAD_PAGES = [dict(k=None), dict(v=None), dict(k=A + 8), dict(v=A + 4), dict(dtype=3), dict(dtype=-1), dict(n_kv=0), dict(n_kv=129),
-             dict(page_size=0), dict(page_size=8), dict(page_size=48), dict(page_size=512), dict(n_pages=-1),
+             dict(page_size=0), dict(page_size=8), dict(page_size=48), dict(page_size=512), dict(n_pages=-1), dict(n_pages=0),
              dict(dtype=L.KV_Q8), dict(dtype=L.KV_Q8, k_scale=A), dict(dtype=L.KV_Q8, k_scale=A, v_scale=A + 4),
              dict(page_rows=32), dict(head_rows=16), dict(page_rows=16, head_rows=8), dict(page_rows=-32, head_rows=16),
              dict(page_rows=24, head_rows=16), dict(page_rows=32, head_rows=24),
