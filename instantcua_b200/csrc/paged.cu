@@ -154,24 +154,36 @@ bool q_type_fits(int dtype, int kvd) {
     return (dtype == ICUA_DT_F16 && kvd != ICUA_KV_BF16) || (dtype == ICUA_DT_BF16 && kvd != ICUA_KV_F16);
 }
 
-template <typename T, bool Q8, int MT>
-cudaError_t launch_attn(const PagedAttnParams& p, int dev, cudaStream_t st) {
-    const int smem = pa_smem(Q8, MT, 1);
-    cudaError_t e = allow_smem<paged_attn_kernel<T, Q8, MT, 1>>(smem, dev);
-    if (e != cudaSuccess) return e;
-    const int ctas = std::min(PA_MAX_CTAS, pa_ctas(Q8, MT, 1) * sm_count(dev));
-    paged_attn_kernel<T, Q8, MT, 1><<<ctas, 32 * pa_warps(1), smem, st>>>(p);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+// A launch that may start while the kernel before it still runs (which it waits for itself).
+template <typename P>
+cudaError_t launch_beside(void (*kernel)(const P), int grid, int block, int smem, cudaStream_t st, const P& p) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(PJ_WARPS * 32);
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_attn_join_kernel<T>, p);
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+// beside: the launch before this one in the stream is the same call's tensor-core kernel.
+template <typename T, bool Q8, int MT>
+cudaError_t launch_attn(const PagedAttnParams& p, bool beside, int dev, cudaStream_t st) {
+    const int smem = pa_smem(Q8, MT, 1);
+    cudaError_t e = allow_smem<paged_attn_kernel<T, Q8, MT, 1>>(smem, dev);
+    if (e != cudaSuccess) return e;
+    const int ctas = std::min(PA_MAX_CTAS, pa_ctas(Q8, MT, 1) * sm_count(dev));
+    if (beside) {
+        e = launch_beside(paged_attn_kernel<T, Q8, MT, 1>, ctas, 32 * pa_warps(1), smem, st, p);
+    } else {
+        paged_attn_kernel<T, Q8, MT, 1><<<ctas, 32 * pa_warps(1), smem, st>>>(p);
+        e = cudaGetLastError();
+    }
+    return e != cudaSuccess ? e : launch_beside(paged_attn_join_kernel<T>, ctas, PJ_WARPS * 32, 0, st, p);
 }
 
 // One cluster per (sequence, kv head), one launch.
@@ -196,15 +208,15 @@ cudaError_t launch_attn_cluster(const PagedAttnParams& p, int dev, cudaStream_t 
 }
 
 template <int MT>
-cudaError_t launch_attn_rows(const PagedAttnParams& p, bool f16, bool q8, bool cluster, int dev, cudaStream_t st) {
+cudaError_t launch_attn_rows(const PagedAttnParams& p, bool f16, bool q8, bool cluster, bool beside, int dev, cudaStream_t st) {
     if constexpr (MT == 1)
         if (cluster)
             return q8    ? (f16 ? launch_attn_cluster<__half, true>(p, dev, st) : launch_attn_cluster<__nv_bfloat16, true>(p, dev, st))
                    : f16 ? launch_attn_cluster<__half, false>(p, dev, st)
                          : launch_attn_cluster<__nv_bfloat16, false>(p, dev, st);
-    return q8    ? (f16 ? launch_attn<__half, true, MT>(p, dev, st) : launch_attn<__nv_bfloat16, true, MT>(p, dev, st))
-           : f16 ? launch_attn<__half, false, MT>(p, dev, st)
-                 : launch_attn<__nv_bfloat16, false, MT>(p, dev, st);
+    return q8    ? (f16 ? launch_attn<__half, true, MT>(p, beside, dev, st) : launch_attn<__nv_bfloat16, true, MT>(p, beside, dev, st))
+           : f16 ? launch_attn<__half, false, MT>(p, beside, dev, st)
+                 : launch_attn<__nv_bfloat16, false, MT>(p, beside, dev, st);
 }
 
 // Sequences with up to PA_ROWS_FEW query rows per kv head go through the warp-MMA kernel, more rows
@@ -233,16 +245,7 @@ cudaError_t launch_attn_tc(const PagedTcParams& p, int tiles, int dev, cudaStrea
     if (e != cudaSuccess) return e;
     paged_attn_tc_kernel<T, Q8><<<tiles * p.pages.n_kv * p.n_split, PC_THREADS, PcSmem<Q8>::alloc, st>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess || p.n_split == 1) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tiles * p.pages.n_kv * 8);
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_attn_tc_join_kernel<T>, p);
+    return launch_beside(paged_attn_tc_join_kernel<T>, tiles * p.pages.n_kv * 8, 256, 0, st, p);
 }
 
 constexpr size_t PA_SCRATCH = PA_MAX_CTAS * (2 * PA_PART * sizeof(float) + sizeof(PaSplit));
@@ -364,6 +367,7 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
     cudaStream_t s = (cudaStream_t)stream;
     const bool f16 = a->dtype == ICUA_DT_F16, q8 = pages->dtype == ICUA_KV_Q8;
     cudaError_t e = cudaSuccess;
+    bool tc_ran = false;
     const bool tc = (int64_t)seqs->max_q * p.group > PA_ROWS_FEW;
     // A batch whose sequences all seem to bring max_q tokens goes there whole, one launch less (a shorter
     // sequence that it holds all the same is then a tile like any other).
@@ -383,7 +387,8 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
         c.err = err_dev;
         const TcGrid g = tc_grid(seqs, pages->n_kv, p.group, c.min_rows, sm_count(dev));
         c.n_split = g.n_split;
-        if (g.tiles > 0)
+        tc_ran = g.tiles > 0;
+        if (tc_ran)
             e = q8 ? (f16 ? launch_attn_tc<__half, true>(c, g.tiles, dev, s) : launch_attn_tc<__nv_bfloat16, true>(c, g.tiles, dev, s))
                 : f16 ? launch_attn_tc<__half, false>(c, g.tiles, dev, s)
                       : launch_attn_tc<__nv_bfloat16, false>(c, g.tiles, dev, s);
@@ -397,7 +402,7 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
         const bool cluster = one_tile && seqs->max_kv <= PA_CLUSTER_KEYS &&
                              (int64_t)seqs->n_seqs * pages->n_kv * PA_CLUSTER <= sm_count(dev);
         if (cluster) p.max_rows = 16;
-        e = one_tile ? launch_attn_rows<1>(p, f16, q8, cluster, dev, s) : launch_attn_rows<2>(p, f16, q8, false, dev, s);
+        e = one_tile ? launch_attn_rows<1>(p, f16, q8, cluster, false, dev, s) : launch_attn_rows<2>(p, f16, q8, false, tc_ran, dev, s);
     }
     return e == cudaSuccess ? ICUA_OK : cuda_fail("icua_attn_paged", e);
 }

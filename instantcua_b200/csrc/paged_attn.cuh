@@ -259,7 +259,10 @@ __global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_
         }
         if (tid == 0) p.split[blockIdx.x] = sp;
         pdl_launch_dependents();
-        if (x0 >= x1) return;
+        if (x0 >= x1) {
+            pdl_wait();  // (see the end)
+            return;
+        }
         auto at = [&](uint32_t x) {  // the first block at or behind unit x
             Cursor c;
             c.s = pa_find(pre, p.seqs.n_seqs, x);
@@ -773,6 +776,9 @@ __global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_
         again = !at_end(c);
     }
     cp_async_wait<0>();
+    // A mixed batch's tensor-core kernel may still run: this grid then started beside it (they share no rows) and
+    // is not done before it, so that whatever follows in the stream comes after both.
+    if (CL == 1) pdl_wait();
 }
 
 // Folds the parts of the items that more than one CTA of paged_attn_kernel worked on: CTA c takes the item
