@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
                 ahead[0] = entry(j + 1, 0);
                 ahead[1] = entry(j + 1, 1);
                 load(rv, p.pages.v, row, left);
-                const uint32_t mine = row[lane >> 4];
+                const uint32_t mine = lane < 16 ? row[0] : row[1];
                 const bool rl = mine != 0xffffffffu && lane < left;
                 const float ksc = rl ? p.pages.ks[mine + (lane & 15)] : 0.f, vsc = rl ? p.pages.vs[mine + (lane & 15)] : 1.f;
                 if (!(ok = room())) break;
@@ -451,8 +451,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
                     float* f = reinterpret_cast<float*>(smem + S::c_off) + (i & 3) * 384 + 32 * w + lane;
                     const float vs = vsc < 1e-37f ? 1e-37f : vsc;
                     f[0] = ksc * p.scale_log2;
-                    f[128] = log2f(vs);
-                    f[256] = vs == vs ? 1.0f / vs : 0.f;
+                    f[128] = lg2_approx(vs);
+                    f[256] = vs == vs ? rcp_approx(vs) : 0.f;
                     mbar_arrive(&c_full[i & 3]);
                 }
                 fence_proxy_async_smem();
@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
         // ---- softmax ---------------------------------------------------------------------------------
         const int hf = warp >> 2, quarter = warp & 3;
         const int R = t.row0 + 128 * hf + 32 * quarter + lane;
-        const int lim = R < rows ? t.kv - t.n + R / G : -1;
+        const int lim = t.kv - t.n + min(R, rows - 1) / G;  // (rows past the end: the last one's, never stored)
         const int nb = half_blocks(hf);
         const uint32_t s_tm = tmem + 128 * hf + ((uint32_t)(32 * quarter) << 16), o_tm = s_tm + 256;
         float m = -INFINITY;
