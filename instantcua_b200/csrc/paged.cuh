@@ -192,7 +192,8 @@ __device__ __forceinline__ void store4(T* p, const float* x) {
 // A CTA takes TOK tokens: a warp each looks its sequence, position and page up, then every token's vectors
 // are dealt to 16 / TOK half-warps, each with its token's rotation row and the norm weights in registers and
 // four vectors' loads in flight.  Bound: HBM for many tokens (each row is read once and written once; TOK = 4
-// shares the lookups), latency for few (TOK = 1).
+// shares the lookups), latency for few (TOK = 1).  Measured on a B200: 13,081 tokens, 32:8 heads, bf16 into q8, and
+// their rows read back by the kernel below, 86 us = 4.4 TB/s (6.54 by copy).
 template <typename TI, typename TQ, int KVD, int TOK>
 __global__ void __launch_bounds__(256, sizeof(TI) == 4 ? 3 : 4) kv_write_kernel(const KvWriteParams p) {
     using TC = typename std::conditional<KVD == KV_BF16, __nv_bfloat16, __half>::type;
@@ -355,7 +356,8 @@ struct KvReadParams {
 
 // value = code * scale (q8) or the stored 16-bit value, one rounding to the output type.  A row of a
 // position that the sequence does not have, or of a table entry that names no page, reads as zeros.
-// Bound: HBM; a half-warp has VPT rows of one token in flight.
+// Bound: HBM; a half-warp has VPT rows of one token in flight (four where that leaves two CTAs per SM).  Measured
+// on a B200: 127,780 tokens, 8 kv heads, q8 to fp16, 139 us = 5.7 TB/s (6.54 by copy).
 template <typename TO, int KVD, int VPT>
 __global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p) {
     using TC = typename std::conditional<KVD == KV_BF16, __nv_bfloat16, __half>::type;

@@ -149,6 +149,11 @@ ATTN = [
     ([500], [2777], dict(n_kv=1, n_q=1, ps=32)),
     ([300, 33], [300, 5000], dict(n_kv=8, n_q=16, layout="lines")),
     ([1024], [1024], dict(n_kv=2, n_q=8, ps=128)),
+    # tokens without a position among those that have one, in a draft and in a chunk
+    ([9, 3, 2], [4, 0, 50], dict(n_kv=2, n_q=6)),
+    ([100, 70, 300], [40, 0, 270], dict(n_kv=2, n_q=8)),
+    # the widest groups: 256 query rows from one token
+    ([1, 3], [200, 1000], dict(n_kv=1, n_q=256)),
 ]
 
 
