@@ -156,9 +156,9 @@ bool q_type_fits(int dtype, int kvd) {
 
 // A launch that may start while the kernel before it still runs (which it waits for itself).
 template <typename P>
-cudaError_t launch_beside(void (*kernel)(const P), int grid, int block, int smem, cudaStream_t st, const P& p) {
+cudaError_t launch_beside(void (*kernel)(const P), dim3 grid, int block, int smem, cudaStream_t st, const P& p) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(block);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -183,7 +183,7 @@ cudaError_t launch_attn(const PagedAttnParams& p, bool beside, int dev, cudaStre
         paged_attn_kernel<T, Q8, MT, 1><<<ctas, 32 * pa_warps(1), smem, st>>>(p);
         e = cudaGetLastError();
     }
-    return e != cudaSuccess ? e : launch_beside(paged_attn_join_kernel<T>, ctas, PJ_WARPS * 32, 0, st, p);
+    return e != cudaSuccess ? e : launch_beside(paged_attn_join_kernel<T>, dim3(ctas, PJ_GROUPS), PJ_WARPS * 32, 0, st, p);
 }
 
 // One cluster per (sequence, kv head), one launch.
@@ -223,8 +223,9 @@ cudaError_t launch_attn_rows(const PagedAttnParams& p, bool f16, bool q8, bool c
 // through the tensor-core kernel.  (28 rows, 24 sequences of about 2,400 positions: 58 us there, 96 us on the
 // tensor core.  With 64 as the border the sequences of a mixed batch that have 33 to 64 rows go through the
 // first kernel's tiles of 32 twice: 47.1 against 45.3 us for 12 sequences of 1 to 600 tokens.)
-// Up to PA_CLUSTER_KEYS positions a cluster per item serves small batches (4,096 positions, 8 kv heads: 10.3 us, 12.3
-// as a line with a join; the eight CTAs of a cluster reach about two thirds of the line's HBM rate beyond).
+// Up to PA_CLUSTER_KEYS positions a cluster per item serves small batches.  (One token, 8 kv heads, bf16, in a
+// graph, cluster against line and join: 512 positions 5.8 / 7.7 us, 2,048 7.1 / 8.6, 4,096 8.9 / 10.8, 8,192 12.7 /
+// 12.4, 32,768 36.6 / 30.1; with fewer heads the line, which always has every SM, catches up earlier.)
 constexpr int PA_ROWS_FEW = 32;
 constexpr int PA_CLUSTER_KEYS = 4096;
 

@@ -788,10 +788,10 @@ __global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_
 }
 
 // Folds the parts of the items that more than one CTA of paged_attn_kernel worked on: CTA c takes the item
-// that c began and did not end.  Eight warps: with few rows several warps share one (each takes every W-th
-// part, eight in flight) and meet in shared memory; the grouping depends on the sizes alone, so the bits do
-// too.
-constexpr int PJ_WARPS = 8;
+// that c began and did not end, a quarter of its rows each (blockIdx.y: a long item has dozens of parts).  Eight
+// warps: with few rows several warps share one (each takes every W-th part, eight in flight) and meet in
+// shared memory; the grouping depends on the sizes alone, so the bits do too.
+constexpr int PJ_WARPS = 8, PJ_GROUPS = 4;
 template <typename T>
 __global__ void __launch_bounds__(PJ_WARPS * 32) paged_attn_join_kernel(const PagedAttnParams p) {
     __shared__ float4 acc_s[PJ_WARPS][32];
@@ -799,15 +799,16 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_attn_join_kernel(const Pa
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.group;
     pdl_wait();
     const PaSplit sp = p.split[blockIdx.x];
-    if (sp.n_parts == 0) return;
-    int log_r = 0;  // rows in a round, a power of two; W warps a row
-    while (log_r < 3 && (1 << log_r) < sp.rows) ++log_r;
+    const int group = (sp.rows + PJ_GROUPS - 1) / PJ_GROUPS, lo = blockIdx.y * group, hi = min(sp.rows, lo + group);
+    if (sp.n_parts == 0 || lo >= hi) return;
+    int log_r = 0;  // rows at a time, a power of two; W warps a row
+    while (log_r < 3 && (1 << log_r) < hi - lo) ++log_r;
     const int W = PJ_WARPS >> log_r, piece = warp >> log_r;
-    for (int r0 = 0; r0 < sp.rows; r0 += 1 << log_r) {
+    for (int r0 = lo; r0 < hi; r0 += 1 << log_r) {
         const int r = r0 + (warp & ((1 << log_r) - 1));
         float m = -INFINITY, l = 0.f;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < sp.rows) {
+        if (r < hi) {
             for (int k0 = piece; k0 < sp.n_parts; k0 += 8 * W) {
                 float pm[8], pl[8];
                 float4 v[8];
@@ -841,7 +842,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_attn_join_kernel(const Pa
                     }
             }
         }
-        if (W > 1) {  // (one round: the rows are fewer than the warps)
+        if (W > 1) {  // (once: the rows are fewer than the warps)
             acc_s[warp][lane] = a;
             if (lane == 0) {
                 ml_s[warp][0] = m;
@@ -863,7 +864,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_attn_join_kernel(const Pa
                     a.w = a.w * f0 + v.w * f1;
                 }
         }
-        if (piece == 0 && r < sp.rows) {
+        if (piece == 0 && r < hi) {
             const float il = m == -INFINITY ? 0.f : 1.0f / l;
             const int rr = sp.first + r;
             T* dst = reinterpret_cast<T*>(p.out) + (sp.q0 + rr / G) * p.out_stride + (sp.h * G + rr % G) * HD + 4 * lane;

@@ -188,8 +188,9 @@ struct PcTile {
     int j0, j1, last;        // blocks of keys [j0, j1); the last key any row sees
 };
 
-// The y-th tile of the batch (later tiles of a sequence, which see more keys, come first), found by one
-// warp.  False past the last one.
+// The y-th tile of the batch, found by one warp: the last tile of every sequence (they see the most keys), then
+// the last but one of each, and so on, 32 sequences at a time; CTAs start in this order, so the long ones do
+// first.  False past the last one.
 __device__ __forceinline__ bool pc_find(const SeqsView& S, int ps_shift, int G, int min_rows, int y, int lane, PcTile& t, int* err) {
     int before = 0;
     for (int s0 = 0; s0 < S.n_seqs; s0 += 32) {
@@ -197,23 +198,24 @@ __device__ __forceinline__ bool pc_find(const SeqsView& S, int ps_shift, int G, 
         if (s0 + lane < S.n_seqs) q = load_seq(S, ps_shift, s0 + lane, err);
         const int rows = q.n * G;
         const int tiles = rows > min_rows ? (rows + PC_ROWS - 1) / PC_ROWS : 0;
-        int x = tiles;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int z = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += z;
-        }
-        const int all = __shfl_sync(0xffffffffu, x, 31);
+        const int all = __reduce_add_sync(0xffffffffu, tiles);
         if (y < before + all) {
-            const unsigned b = __ballot_sync(0xffffffffu, y < before + x);
-            const int src = __ffs(b) - 1;
+            // the turn: the most r with y at or behind the first r tiles of every sequence
+            int lo = 0, hi = __reduce_max_sync(0xffffffffu, tiles);
+            while (hi - lo > 1) {
+                const int r = (lo + hi) >> 1;
+                if (y - before >= __reduce_add_sync(0xffffffffu, min(tiles, r))) lo = r;
+                else hi = r;
+            }
+            int i = y - before - __reduce_add_sync(0xffffffffu, min(tiles, lo));
+            unsigned has = __ballot_sync(0xffffffffu, tiles > lo);
+            for (; i > 0; --i) has &= has - 1;
+            const int src = __ffs(has) - 1;
             t.s = s0 + src;
             t.q0 = __shfl_sync(0xffffffffu, q.q0, src);
             t.n = __shfl_sync(0xffffffffu, q.n, src);
             t.kv = __shfl_sync(0xffffffffu, q.kv, src);
-            const int first = before + __shfl_sync(0xffffffffu, x - tiles, src);
-            const int cnt = __shfl_sync(0xffffffffu, tiles, src);
-            t.row0 = (cnt - 1 - (y - first)) * PC_ROWS;
+            t.row0 = (__shfl_sync(0xffffffffu, tiles, src) - 1 - lo) * PC_ROWS;
             return true;
         }
         before += all;
