@@ -207,16 +207,23 @@ cudaError_t launch_attn_cluster(const PagedAttnParams& p, int dev, cudaStream_t 
     return cudaLaunchKernelEx(&cfg, paged_attn_kernel<T, Q8, 1, PA_CLUSTER>, p);
 }
 
-template <int MT>
-cudaError_t launch_attn_rows(const PagedAttnParams& p, bool f16, bool q8, bool cluster, bool beside, int dev, cudaStream_t st) {
-    if constexpr (MT == 1)
-        if (cluster)
-            return q8    ? (f16 ? launch_attn_cluster<__half, true>(p, dev, st) : launch_attn_cluster<__nv_bfloat16, true>(p, dev, st))
-                   : f16 ? launch_attn_cluster<__half, false>(p, dev, st)
-                         : launch_attn_cluster<__nv_bfloat16, false>(p, dev, st);
-    return q8    ? (f16 ? launch_attn<__half, true, MT>(p, beside, dev, st) : launch_attn<__nv_bfloat16, true, MT>(p, beside, dev, st))
-           : f16 ? launch_attn<__half, false, MT>(p, beside, dev, st)
-                 : launch_attn<__nv_bfloat16, false, MT>(p, beside, dev, st);
+// One CTA per (sequence, kv head), one launch.
+template <typename T, bool Q8, int MT>
+cudaError_t launch_attn_cta(const PagedAttnParams& p, bool beside, int dev, cudaStream_t st) {
+    const int smem = pa_smem(Q8, MT, 0), items = p.seqs.n_seqs * p.pages.n_kv;
+    const cudaError_t e = allow_smem<paged_attn_kernel<T, Q8, MT, 0>>(smem, dev);
+    if (e != cudaSuccess) return e;
+    if (beside) return launch_beside(paged_attn_kernel<T, Q8, MT, 0>, dim3(items), 32 * pa_warps(0), smem, st, p);
+    paged_attn_kernel<T, Q8, MT, 0><<<items, 32 * pa_warps(0), smem, st>>>(p);
+    return cudaGetLastError();
+}
+
+enum class Share { line, cta, cluster };
+template <typename T, bool Q8>
+cudaError_t launch_attn_few(const PagedAttnParams& p, Share share, bool one_tile, bool beside, int dev, cudaStream_t st) {
+    if (share == Share::cluster) return launch_attn_cluster<T, Q8>(p, dev, st);
+    if (share == Share::cta) return one_tile ? launch_attn_cta<T, Q8, 1>(p, beside, dev, st) : launch_attn_cta<T, Q8, 2>(p, beside, dev, st);
+    return one_tile ? launch_attn<T, Q8, 1>(p, beside, dev, st) : launch_attn<T, Q8, 2>(p, beside, dev, st);
 }
 
 // Sequences with up to PA_ROWS_FEW query rows per kv head go through the warp-MMA kernel, more rows
@@ -228,6 +235,12 @@ cudaError_t launch_attn_rows(const PagedAttnParams& p, bool f16, bool q8, bool c
 // 12.4, 32,768 36.6 / 30.1; with fewer heads the line, which always has every SM, catches up earlier.)
 constexpr int PA_ROWS_FEW = 32;
 constexpr int PA_CLUSTER_KEYS = 4096;
+// Up to PA_CTA_KEYS a CTA per item serves the others, without the line's counting and its join.  (Single tokens, 8
+// kv heads, bf16 / q8, in a graph, CTA against line: 20 sequences of 64 positions 4.6 / 5.6 against 8.8 / 10.6 us, of
+// 512 11.0 / 13.7 against 14.5 / 17.1, of 1,024 18.2 / 24.2 against 18.6 / 23.7; 256 of 1,024 165 / 144 against 173 /
+// 165.  Beyond, a batch of few items needs the line to fill the GPU, and one long sequence to be shared.)
+constexpr int PA_CTA_KEYS = 1024;
+static_assert(PA_ROWS_FEW <= 32, "the kernel's largest tile holds every item");
 
 // Tiles of the tensor-core kernel: a bound from what the host knows, and the shares of the keys that fill
 // the SMs when the tiles alone do not (two blocks of keys per share at least).
@@ -399,15 +412,15 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
                       : launch_attn_tc<__nv_bfloat16, false>(c, g.tiles, dev, s);
     }
     p.alone = !tc;
-    if (e == cudaSuccess && !all_tc)
-    {
+    if (e == cudaSuccess && !all_tc) {
         const bool one_tile = (int64_t)seqs->max_q * p.group <= 16;
-        // Few items, up to PA_CLUSTER_KEYS keys each: a cluster per item does without the second launch.  Longer
-        // ones want every SM, and more of them fill the GPU by themselves.
-        const bool cluster = one_tile && seqs->max_kv <= PA_CLUSTER_KEYS &&
-                             (int64_t)seqs->n_seqs * pages->n_kv * PA_CLUSTER <= sm_count(dev);
-        if (cluster) p.max_rows = 16;
-        e = one_tile ? launch_attn_rows<1>(p, f16, q8, cluster, false, dev, s) : launch_attn_rows<2>(p, f16, q8, false, tc_ran, dev, s);
+        const bool few = one_tile && (int64_t)seqs->n_seqs * pages->n_kv * PA_CLUSTER <= sm_count(dev);
+        const Share share = few && seqs->max_kv <= PA_CLUSTER_KEYS ? Share::cluster : seqs->max_kv <= PA_CTA_KEYS ? Share::cta : Share::line;
+        if (share != Share::line) p.max_rows = one_tile ? 16 : 32;  // one tile per (sequence, kv head)
+        e = q8 ? (f16 ? launch_attn_few<__half, true>(p, share, one_tile, tc_ran, dev, s)
+                      : launch_attn_few<__nv_bfloat16, true>(p, share, one_tile, tc_ran, dev, s))
+            : f16 ? launch_attn_few<__half, false>(p, share, one_tile, tc_ran, dev, s)
+                  : launch_attn_few<__nv_bfloat16, false>(p, share, one_tile, tc_ran, dev, s);
     }
     return e == cudaSuccess ? ICUA_OK : cuda_fail("icua_attn_paged", e);
 }

@@ -27,7 +27,7 @@
 //
 // Measured on a B200 (6.54 TB/s by copy): 48 single tokens over 3 .. 16,000 positions, 32:8 heads, bf16, 76 us =
 // 5.5 TB/s; 64 over about 2,000 positions, 16:8 heads, q8, 72 us = 3.8 TB/s, bound by the conversions (half of
-// the issue slots at three warps per scheduler); 24 drafts of 7 tokens, 32:8 heads, fp16, 56 us = 3.5 TB/s, bound
+// the issue slots at three warps per scheduler); 24 drafts of 7 tokens, 32:8 heads, fp16, 54 us = 3.6 TB/s, bound
 // by latency (the two tiles' registers leave two warps per scheduler); one token over 4,096 positions, 16:8
 // heads, bf16, in a cluster per kv head 10.3 us against 12.3 us dealt as a line and joined.
 #pragma once
@@ -76,7 +76,7 @@ constexpr int pa_ctas(bool q8, int mt, int cl) { return cl > 1 ? 1 : q8 && mt ==
 constexpr int pa_ns(bool q8, int mt, int cl) { return pa_ctas(q8, mt, cl) == 2 ? 3 : 2; }
 constexpr bool pa_q_in_smem(bool q8, int mt) { return mt > 1 || q8; }
 constexpr int pa_smem(bool q8, int mt, int cl) {
-    return pa_warps(cl) * pa_ns(q8, mt, cl) * pa_slot(q8) + (pa_q_in_smem(q8, mt) ? mt * 16 * 2 * HD : 0) + (cl > 1 ? 0 : (PA_MAX_SEQS + 1) * 4);
+    return pa_warps(cl) * pa_ns(q8, mt, cl) * pa_slot(q8) + (pa_q_in_smem(q8, mt) ? mt * 16 * 2 * HD : 0) + (cl == 1 ? (PA_MAX_SEQS + 1) * 4 : 0);
 }
 
 __device__ __forceinline__ void cluster_barrier() {
@@ -220,11 +220,14 @@ struct PaDeal {
 };
 
 // MT: tiles of sixteen query rows per item that share every K and V fragment.
-// CL > 1 (few sequences of moderate length): no line; the cluster's CL CTAs share one item, (sequence, kv
-// head) of the cluster's number, and join its parts through distributed shared memory.  One launch and no
-// workspace, for calls whose time is latency.
+// CL = 1: the line and a join.  CL > 1 (few sequences of moderate length): the cluster's CL CTAs share one item,
+// (sequence, kv head) of the cluster's number, and join its parts through distributed shared memory.  CL = 0
+// (many short sequences): a CTA per item.  The last two are one launch without workspace, for calls whose
+// time is latency.
 template <typename T, bool Q8, int MT, int CL>
 __global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_attn_kernel(const PagedAttnParams p) {
+    constexpr bool LINE = CL == 1;
+    constexpr int CN = CL > 1 ? CL : 1;  // CTAs that share an item
     constexpr int PA_WARPS = pa_warps(CL), PA_THREADS = 32 * PA_WARPS, PA_NS = pa_ns(Q8, MT, CL);
     constexpr bool QS = pa_q_in_smem(Q8, MT);
     constexpr int KEYS = pa_keys(Q8), BLOCK = pa_block(Q8, CL), SLOT = pa_slot(Q8), NT = KEYS / 8, ROWS = 16 * MT;
@@ -244,7 +247,7 @@ __global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_
     };
     auto work_of = [&](int s, int* err) { return pa_work(p.seqs, ps_shift, n_kv, G, p.max_rows, ROWS, BLOCK, s, err, p.alone != 0); };
     Cursor f{}, end{};  // this CTA's first block, and the one after its last
-    if (CL == 1) {
+    if (LINE) {
         const uint32_t total = pa_prefix<PA_THREADS>(p.seqs, ps_shift, n_kv, G, p.max_rows, ROWS, BLOCK, pre, warp_tot,
                                                      blockIdx.x == 0 ? p.err : nullptr, p.alone != 0);
         const PaDeal deal(total, gridDim.x);
@@ -282,14 +285,17 @@ __global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_
         if (x1 < total) end = at(x1);
         else end.s = -1;
     } else {
-        const int item = blockIdx.x / CL, rank = blockIdx.x % CL;
+        const int item = blockIdx.x / CN, rank = blockIdx.x % CN;
         f.s = item / n_kv;
         f.w = work_of(f.s, rank == 0 && item % n_kv == 0 ? p.err : nullptr);
-        if (f.w.items == 0) return;  // (the whole cluster)
-        f.item = item % n_kv;        // (one tile: max_rows is 16)
+        if (f.w.items == 0) {  // (the whole cluster)
+            if (CL == 0) pdl_wait();  // (see the end)
+            return;
+        }
+        f.item = item % n_kv;  // (one tile: max_rows is ROWS)
         end = f;
-        f.b = (int)((long long)f.w.nb * rank / CL);
-        end.b = (int)((long long)f.w.nb * (rank + 1) / CL);
+        f.b = (int)((long long)f.w.nb * rank / CN);
+        end.b = (int)((long long)f.w.nb * (rank + 1) / CN);
     }
     auto at_end = [&](const Cursor& c) { return c.s == end.s && c.item == end.item && c.b == end.b; };
     auto next_item = [&](Cursor& c) {  // the next one's first block; behind the last item: s = -1, as in `end`
@@ -384,7 +390,7 @@ __global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_
                     }
                 }
             }
-            if (++f.b == f.w.nb && (CL == 1 || f.b != end.b)) next_item(f);
+            if (++f.b == f.w.nb && (LINE || f.b != end.b)) next_item(f);
             more = !at_end(f);
             look();
         }
@@ -394,7 +400,7 @@ __global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_
     for (int i = 0; i < PA_NS; ++i) fetch(i);
 
     int slot = 0;
-    bool again = CL > 1 || !at_end(c);  // (a CTA of a cluster without a block still takes part in the join)
+    bool again = !LINE || !at_end(c);  // (a CTA of a cluster without a block still takes part in the join)
     while (again) {
         const int h = c.item / c.w.tiles, tile = c.item - h * c.w.tiles;
         const int b0 = c.b, b1 = c.s == end.s && c.item == end.item ? end.b : c.w.nb;
@@ -732,13 +738,14 @@ __global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_
                     ml_c[0][rt] = mm;
                     ml_c[1][rt] = ll;
                 }
-                if (CL == 1 && !whole && tid % TPR == 0) {
+                if (LINE && !whole && tid % TPR == 0) {
                     pt[PA_ROWS_MAX * HD + rt] = mm;
                     pt[PA_ROWS_MAX * HD + PA_ROWS_MAX + rt] = ll;
                 }
             }
         }
-        if (CL > 1) {
+        if (CL == 0) break;  // (the one item is whole, and nothing more was requested)
+        if constexpr (CL > 1) {
             // every CTA's part is in its own shared memory: CTA `rank` folds columns [16 rank, 16 rank + 16) of all
             cluster_barrier();
             const int r = tid >> 3, rr = tile * ROWS + r, rank = blockIdx.x % CL;
@@ -784,7 +791,7 @@ __global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_
     cp_async_wait<0>();
     // A mixed batch's tensor-core kernel may still run: this grid then started beside it (they share no rows) and
     // is not done before it, so that whatever follows in the stream comes after both.
-    if (CL == 1) pdl_wait();
+    pdl_wait();
 }
 
 // Folds the parts of the items that more than one CTA of paged_attn_kernel worked on: CTA c takes the item

@@ -410,3 +410,16 @@ def test_prompts_then_decoding_together(cache, typ):
         step_size = qkv.view(c.total, -1, HD)[:, n_q + n_kv:].abs().amax(-1, keepdim=True)
         half = 0.502 / 127 if cache == "q8" else torch.finfo(cache).eps / 2
         assert ((v32 - qkv.view(c.total, -1, HD)[:, n_q + n_kv:]).abs() <= half * step_size).all()
+
+
+@pytest.mark.parametrize("cache,typ", TYPES, ids=name)
+@pytest.mark.parametrize("n,kv", [([1] * 5, [700, 3, 5000, 64, 0]), ([6, 1, 3], [400, 6000, 3]), ([1], [9000]),
+                                  ([90, 5, 1, 0], [90, 3000, 12, 7])], ids=str)
+def test_the_length_hint_changes_no_result(n, kv, cache, typ):
+    """max_kv only steers the split: far too small and far too large values give the same attention."""
+    c = Cache(n, kv, cache=cache, typ=typ, n_kv=2, n_q=8).fill(scale=2.0)
+    q = (c.randn(c.total, 8, HD) * 2).to(typ)
+    want, bound = c.attend64(q)
+    for hint in (0, 1, 1024, 4096, 1 << 20):
+        check_close(c.attend(q, max_kv=hint), want, bound, f"max_kv {hint}")
+    assert c.flags() == 0
