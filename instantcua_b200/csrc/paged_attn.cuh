@@ -795,10 +795,10 @@ __global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_
 }
 
 // Folds the parts of the items that more than one CTA of paged_attn_kernel worked on: CTA c takes the item
-// that c began and did not end, a quarter of its rows each (blockIdx.y: a long item has dozens of parts).  Eight
+// that c began and did not end, one of gridDim.y groups of its rows each (a long item has dozens of parts).  Eight
 // warps: with few rows several warps share one (each takes every W-th part, eight in flight) and meet in
 // shared memory; the grouping depends on the sizes alone, so the bits do too.
-constexpr int PJ_WARPS = 8, PJ_GROUPS = 4;
+constexpr int PJ_WARPS = 8;
 template <typename T>
 __global__ void __launch_bounds__(PJ_WARPS * 32) paged_attn_join_kernel(const PagedAttnParams p) {
     __shared__ float4 acc_s[PJ_WARPS][32];
@@ -806,7 +806,7 @@ __global__ void __launch_bounds__(PJ_WARPS * 32) paged_attn_join_kernel(const Pa
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.group;
     pdl_wait();
     const PaSplit sp = p.split[blockIdx.x];
-    const int group = (sp.rows + PJ_GROUPS - 1) / PJ_GROUPS, lo = blockIdx.y * group, hi = min(sp.rows, lo + group);
+    const int group = (sp.rows + gridDim.y - 1) / gridDim.y, lo = blockIdx.y * group, hi = min(sp.rows, lo + group);
     if (sp.n_parts == 0 || lo >= hi) return;
     int log_r = 0;  // rows at a time, a power of two; W warps a row
     while (log_r < 3 && (1 << log_r) < hi - lo) ++log_r;

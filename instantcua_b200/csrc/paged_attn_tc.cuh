@@ -201,15 +201,20 @@ __device__ __forceinline__ bool pc_find(const SeqsView& S, int ps_shift, int G, 
         const int all = __reduce_add_sync(0xffffffffu, tiles);
         if (y < before + all) {
             // the turn: the most r with y at or behind the first r tiles of every sequence
-            int lo = 0, hi = __reduce_max_sync(0xffffffffu, tiles);
-            while (hi - lo > 1) {
-                const int r = (lo + hi) >> 1;
-                if (y - before >= __reduce_add_sync(0xffffffffu, min(tiles, r))) lo = r;
-                else hi = r;
+            unsigned has = __ballot_sync(0xffffffffu, tiles > 0);
+            int lo = y - before;  // (one sequence: its tiles in turn)
+            if (has & (has - 1)) {
+                int hi = __reduce_max_sync(0xffffffffu, tiles);
+                lo = 0;
+                while (hi - lo > 1) {
+                    const int r = (lo + hi) >> 1;
+                    if (y - before >= __reduce_add_sync(0xffffffffu, min(tiles, r))) lo = r;
+                    else hi = r;
+                }
+                int i = y - before - __reduce_add_sync(0xffffffffu, min(tiles, lo));
+                has = __ballot_sync(0xffffffffu, tiles > lo);
+                for (; i > 0; --i) has &= has - 1;
             }
-            int i = y - before - __reduce_add_sync(0xffffffffu, min(tiles, lo));
-            unsigned has = __ballot_sync(0xffffffffu, tiles > lo);
-            for (; i > 0; --i) has &= has - 1;
             const int src = __ffs(has) - 1;
             t.s = s0 + src;
             t.q0 = __shfl_sync(0xffffffffu, q.q0, src);
