@@ -408,7 +408,8 @@ uint64_t icua_attn_paged_scratch_bytes(const icua_kv_pages* pages, const icua_kv
 /* Causal attention of every new token over its sequence's cache up to its own position (which
  * icua_kv_write has filled): one token per sequence (decode), drafts, chunks of a prompt and whole
  * prompts, together in one call.  Scores, softmax and sums in fp32, probabilities rounded to the
- * type of q.  Rows of a 16-bit cache behind a sequence's end are never used; rows of its own new
+ * type of q (the scales of a q8 cache round nothing; a V scale below 1e-30 counts as 1e-30).  Rows of a
+ * 16-bit cache behind a sequence's end are never used; rows of its own new
  * tokens must be finite, since a later token's infinity or NaN reaches the earlier ones of the same
  * call (0 x inf).  A token without a position (kv_len < n) gets zeros. */
 icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs, const icua_attn_paged_args* args,

@@ -116,12 +116,28 @@ cudaError_t allow_smem(int bytes, int dev) {
 // four vectors per half-warp where that still leaves two CTAs (of 16 half-warps) per SM
 int vectors_per_unit(int64_t tokens, int n_vec, int n_sm) { return tokens * ((n_vec + 3) / 4) >= 2ll * 16 * n_sm ? 4 : 1; }
 
+// beside: the launch may start while the kernel before it still runs (which it waits for itself).
+template <typename P>
+cudaError_t launch_on(void (*kernel)(const P), dim3 grid, int block, int smem, cudaStream_t st, bool beside, const P& p) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = beside ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 template <typename TI, typename TQ, int KVD>
 cudaError_t launch_write(const KvWriteParams& p, int n_sm, cudaStream_t st) {
     // four tokens a CTA once that leaves two CTAs per SM
-    if (p.seqs.total_q >= 8 * n_sm) kv_write_kernel<TI, TQ, KVD, 4><<<(p.seqs.total_q - 1) / 4 + 1, 256, 0, st>>>(p);
-    else kv_write_kernel<TI, TQ, KVD, 1><<<p.seqs.total_q, 256, 0, st>>>(p);
-    return cudaGetLastError();
+    if (p.seqs.total_q >= 8 * n_sm)
+        return launch_on(kv_write_kernel<TI, TQ, KVD, 4>, dim3((p.seqs.total_q - 1) / 4 + 1), 256, 0, st, false, p);
+    return launch_on(kv_write_kernel<TI, TQ, KVD, 1>, dim3(p.seqs.total_q), 256, 0, st, false, p);
 }
 
 template <typename TI>
@@ -137,9 +153,7 @@ cudaError_t launch_read_one(KvReadParams& p, int n_sm, cudaStream_t st) {
     const int vpt = vectors_per_unit(p.seqs.total_q, n_vec, n_sm);
     p.n_groups = (n_vec + vpt - 1) / vpt;
     const int64_t grid = ((int64_t)p.seqs.total_q * p.n_groups + 15) / 16;
-    if (vpt == 4) kv_read_kernel<TO, KVD, 4><<<(unsigned)grid, 256, 0, st>>>(p);
-    else kv_read_kernel<TO, KVD, 1><<<(unsigned)grid, 256, 0, st>>>(p);
-    return cudaGetLastError();
+    return launch_on(vpt == 4 ? kv_read_kernel<TO, KVD, 4> : kv_read_kernel<TO, KVD, 1>, dim3((unsigned)grid), 256, 0, st, false, p);
 }
 
 template <typename TO>
@@ -154,22 +168,6 @@ bool q_type_fits(int dtype, int kvd) {
     return (dtype == ICUA_DT_F16 && kvd != ICUA_KV_BF16) || (dtype == ICUA_DT_BF16 && kvd != ICUA_KV_F16);
 }
 
-// A launch that may start while the kernel before it still runs (which it waits for itself).
-template <typename P>
-cudaError_t launch_beside(void (*kernel)(const P), dim3 grid, int block, int smem, cudaStream_t st, const P& p) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
-}
-
 // beside: the launch before this one in the stream is the same call's tensor-core kernel.
 template <typename T, bool Q8, int MT>
 cudaError_t launch_attn(const PagedAttnParams& p, bool beside, int dev, cudaStream_t st) {
@@ -177,16 +175,11 @@ cudaError_t launch_attn(const PagedAttnParams& p, bool beside, int dev, cudaStre
     cudaError_t e = allow_smem<paged_attn_kernel<T, Q8, MT, 1>>(smem, dev);
     if (e != cudaSuccess) return e;
     const int ctas = std::min(PA_MAX_CTAS, pa_ctas(Q8, MT, 1) * sm_count(dev));
-    if (beside) {
-        e = launch_beside(paged_attn_kernel<T, Q8, MT, 1>, ctas, 32 * pa_warps(1), smem, st, p);
-    } else {
-        paged_attn_kernel<T, Q8, MT, 1><<<ctas, 32 * pa_warps(1), smem, st>>>(p);
-        e = cudaGetLastError();
-    }
+    e = launch_on(paged_attn_kernel<T, Q8, MT, 1>, dim3(ctas), 32 * pa_warps(1), smem, st, beside, p);
     // Items in many parts are joined by four CTAs each (12 sequences of up to 34,000 positions, 2 kv heads: 31 -> 25 us);
     // where the parts are few one does, and the launch stays small (64 sequences of 2,000, 8 kv heads: 72 against 74).
     const int groups = p.seqs.n_seqs * p.pages.n_kv * 4 <= ctas ? 4 : 1;
-    return e != cudaSuccess ? e : launch_beside(paged_attn_join_kernel<T>, dim3(ctas, groups), PJ_WARPS * 32, 0, st, p);
+    return e != cudaSuccess ? e : launch_on(paged_attn_join_kernel<T>, dim3(ctas, groups), PJ_WARPS * 32, 0, st, true, p);
 }
 
 // One cluster per (sequence, kv head), one launch.
@@ -216,9 +209,7 @@ cudaError_t launch_attn_cta(const PagedAttnParams& p, bool beside, int dev, cuda
     const int smem = pa_smem(Q8, MT, 0), items = p.seqs.n_seqs * p.pages.n_kv;
     const cudaError_t e = allow_smem<paged_attn_kernel<T, Q8, MT, 0>>(smem, dev);
     if (e != cudaSuccess) return e;
-    if (beside) return launch_beside(paged_attn_kernel<T, Q8, MT, 0>, dim3(items), 32 * pa_warps(0), smem, st, p);
-    paged_attn_kernel<T, Q8, MT, 0><<<items, 32 * pa_warps(0), smem, st>>>(p);
-    return cudaGetLastError();
+    return launch_on(paged_attn_kernel<T, Q8, MT, 0>, dim3(items), 32 * pa_warps(0), smem, st, beside, p);
 }
 
 enum class Share { line, cta, cluster };
@@ -264,9 +255,9 @@ template <typename T, bool Q8>
 cudaError_t launch_attn_tc(const PagedTcParams& p, int tiles, int dev, cudaStream_t st) {
     cudaError_t e = allow_smem<paged_attn_tc_kernel<T, Q8>>(PcSmem<Q8>::alloc, dev);
     if (e != cudaSuccess) return e;
-    paged_attn_tc_kernel<T, Q8><<<tiles * p.pages.n_kv * p.n_split, PC_THREADS, PcSmem<Q8>::alloc, st>>>(p);
-    if ((e = cudaGetLastError()) != cudaSuccess || p.n_split == 1) return e;
-    return launch_beside(paged_attn_tc_join_kernel<T>, tiles * p.pages.n_kv * 8, 256, 0, st, p);
+    e = launch_on(paged_attn_tc_kernel<T, Q8>, dim3(tiles * p.pages.n_kv * p.n_split), PC_THREADS, PcSmem<Q8>::alloc, st, false, p);
+    if (e != cudaSuccess || p.n_split == 1) return e;
+    return launch_on(paged_attn_tc_join_kernel<T>, dim3(tiles * p.pages.n_kv * 8), 256, 0, st, true, p);
 }
 
 constexpr size_t PA_SCRATCH = PA_MAX_CTAS * (2 * PA_PART * sizeof(float) + sizeof(PaSplit));

@@ -528,8 +528,9 @@ __global__ void __launch_bounds__(32 * pa_warps(CL), pa_ctas(Q8, MT, CL)) paged_
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             // a NaN scale (a poisoned row) reaches the rows that see it through the score; a masked
-                            // one adds 0 x 0 to their sums
-                            const float vs = vv[e] < 1e-37f ? 1e-37f : vv[e];
+                            // one adds 0 x 0 to their sums.  Scales below 1e-30 count as that: p' must not fall
+                            // under fp32's range while p / vs still counts in the sum
+                            const float vs = vv[e] < 1e-30f ? 1e-30f : vv[e];
                             const float add = lg2_approx(vs), mul = av[e] * p.scale_log2;
                             inv[2 * nt + e] = vs == vs ? rcp_approx(vs) : 0.f;
 #pragma unroll

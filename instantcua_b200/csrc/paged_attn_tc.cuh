@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
                 {
                     // (block i + 4 is stored after the scores of block i + 2, which come after both halves' softmax of i)
                     float* f = reinterpret_cast<float*>(smem + S::c_off) + (i & 3) * 384 + 32 * w + lane;
-                    const float vs = vsc < 1e-37f ? 1e-37f : vsc;
+                    const float vs = vsc < 1e-30f ? 1e-30f : vsc;
                     f[0] = ksc * p.scale_log2;
                     f[128] = lg2_approx(vs);
                     f[256] = vs == vs ? rcp_approx(vs) : 0.f;

@@ -423,3 +423,19 @@ def test_the_length_hint_changes_no_result(n, kv, cache, typ):
     for hint in (0, 1, 1024, 4096, 1 << 20):
         check_close(c.attend(q, max_kv=hint), want, bound, f"max_kv {hint}")
     assert c.flags() == 0
+
+
+@pytest.mark.parametrize("n", [1, 2, 100])
+def test_v_rows_of_wildly_different_sizes(n):
+    """Half of the probability on a row 10^32 times smaller than the other's: it adds nothing to the result, but it counts."""
+    c = Cache([n], [n + 63], cache="q8", typ=BF16, n_kv=1, n_q=1)
+    total = n + 63
+    ks = torch.zeros(total, 1, HD, device="cuda")
+    vs = torch.ones(total, 1, HD, device="cuda")
+    vs[::2] *= 1e-32
+    c.fill([ks], [vs * 3])
+    q = c.randn(n, 1, HD).bfloat16()
+    out = c.attend(q)
+    pos = torch.arange(63, total, device="cuda")
+    want = 3.0 * ((pos + 1) // 2).double() / (pos + 1).double()
+    assert ((out.double() - want[:, None, None]).abs() <= want[:, None, None] * 2.0 ** -7).all()
