@@ -660,7 +660,9 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
                 }
             }
         }
-        if (ok && nb > 0 && !__all_sync(0xffffffffu, mbar_wait_bounded(&o_full[hf], 0))) ok = false;
+        // The rows go out through the half's q tile: behind its last product or, where no row has a position and so no
+        // product runs, behind the copies that fill the tile.
+        if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(nb > 0 ? &o_full[hf] : q_full, 0))) ok = false;
         tc_fence_after();
         if (!ok) {
             if (lane == 0 && p.err) atomicOr(p.err, ERR_WAIT_PREFILL);

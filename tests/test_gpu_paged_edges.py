@@ -1,0 +1,42 @@
+"""GPU tests of calls of the paged K/V cache operators that the ordinary ones do not make: whole halves of a tile without
+a position, entries that contradict each other far back in a batch, hints and sizes at their ends."""
+import pytest
+import torch
+
+from _paged import Cache, check_close
+
+pytestmark = pytest.mark.gpu
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+TYPES = [(F16, F16), (BF16, BF16), ("q8", F16), ("q8", BF16)]
+
+
+@pytest.fixture(autouse=True)
+def _gpu(require_gpu):
+    pass
+
+
+def name(v):
+    return {F16: "f16", BF16: "bf16", F32: "f32"}.get(v, v) if not isinstance(v, (list, tuple)) else None
+
+
+@pytest.mark.parametrize("cache,typ", TYPES, ids=name)
+@pytest.mark.parametrize("n,kv", [([300], [100]), ([300], [204]), ([200], [0]), ([64, 300, 1], [0, 110, 5]), ([257] * 9, [130] * 9)], ids=str)
+def test_halves_of_a_tile_without_a_position(n, kv, cache, typ):
+    """256 query rows a tile, four heads a token: tiles and halves of tiles whose tokens all lie before the cache's first
+    position get zeros, the rows behind them their attention, also in place and every time.  At most 256 positions: a tile's
+    keys are one share, so that its rows are written where they are computed."""
+    c = Cache(n, kv, cache=cache, typ=typ, n_kv=2, n_q=8, seed=sum(n)).fill()
+    assert max(kv) <= 256
+    q = (c.randn(c.total, 8, 128) * 2).to(typ)
+    want, bound = c.attend64(q)
+    first = c.attend(q, torch.full_like(q, 6.0))
+    check_close(first, want, bound)
+    at = 0
+    for a, b in zip(n, kv):
+        assert (first[at:at + max(0, a - b)] == 0).all()
+        at += a
+    for _ in range(20):
+        same = q.clone()
+        c.attend(same, same)
+        assert torch.equal(same, first)
+    assert c.flags() == 0
