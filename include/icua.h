@@ -330,8 +330,10 @@ icua_status icua_dequant(int32_t fmt, int32_t n_rows, int32_t k, const void* pac
  * ICUA_FLAG_SEQ.  err_dev: optional device int32 that the flags are OR-ed into. */
 enum { ICUA_DT_F32 = 0, ICUA_DT_BF16 = 1, ICUA_DT_F16 = 2 }; /* row types, as icua_gemv's x_dtype */
 /* Third cache type: int8 codes with one fp32 scale per row (position, head): scale = max|x| / 127,
- * code = x / scale to the nearest even; a row of zeros has the scale 1, a row that holds a NaN or an
- * infinity reads back as NaN.  Paged caches only (icua_config.kv_dtype stays 16-bit). */
+ * code = x / scale to the nearest (2^-15 of a step around a tie may go either way); a row of zeros has
+ * the scale 1 (K) or 2^-60 (V), a row that holds a NaN or an infinity reads back as NaN.  Paged caches
+ * only (icua_config.kv_dtype stays 16-bit).  A cache that is filled in another way keeps each V scale
+ * near its row's max|x| / 127, that of a row of zeros far below the others: see icua_attn_paged. */
 enum { ICUA_KV_Q8 = 2 };
 enum { ICUA_FLAG_WAIT = 4, ICUA_FLAG_PAGE = 16, ICUA_FLAG_SEQ = 32 };
 
@@ -408,8 +410,10 @@ uint64_t icua_attn_paged_scratch_bytes(const icua_kv_pages* pages, const icua_kv
 /* Causal attention of every new token over its sequence's cache up to its own position (which
  * icua_kv_write has filled): one token per sequence (decode), drafts, chunks of a prompt and whole
  * prompts, together in one call.  Scores, softmax and sums in fp32, probabilities rounded to the
- * type of q (the scales of a q8 cache round nothing; a V scale below 1e-30 counts as 1e-30).  Rows of a
- * 16-bit cache behind a sequence's end are never used; rows of its own new
+ * type of q.  In a q8 cache a probability is rounded after it was multiplied by its key's V scale, relative to
+ * the largest such product: all products are held as precisely down to 2^-14 (fp16) or 2^-126 (bf16) of it,
+ * smaller ones are off by up to 2^-25 of it in fp16; the sums take them unrounded.  A V scale below 1e-30
+ * counts as 1e-30.  Rows of a 16-bit cache behind a sequence's end are never used; rows of its own new
  * tokens must be finite, since a later token's infinity or NaN reaches the earlier ones of the same
  * call (0 x inf).  A token without a position (kv_len < n) gets zeros. */
 icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs, const icua_attn_paged_args* args,

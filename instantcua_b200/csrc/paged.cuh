@@ -81,6 +81,12 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
     return d;
 }
 
+// Scale of a V row of zeros.  The attention takes its probabilities relative to the largest product of probability and V
+// scale, in 16 bits: with the scale 1 a row that adds nothing would set that maximum and push keys with small V rows
+// under fp16's normal numbers (rows of 1e-5 beside one of zeros: up to 63 % off).  2^-60 is below the scales of values down
+// to 1e-16, and so far above fp32's smallest numbers that the row still counts in the sum beside V rows of up to 1e12.
+constexpr float KV_ZERO_V = 8.673617379884035e-19f;
+
 struct KvWriteParams {
     PagesView pages;
     SeqsView seqs;
@@ -188,7 +194,7 @@ __device__ __forceinline__ void store4(T* p, const float* x) {
 // rotation pairs.  y = x rsqrt(mean x^2 + eps) w, then (y_j c - y_{j+64} s, y_{j+64} c + y_j s), in fp32; q rows
 // are rounded to the output type, k and v rows to the cache type or to int8 codes: scale = max|x| / 127 in fp32
 // and code = x / scale to the nearest even, so a code is off by at most half a step.  A row that holds a NaN
-// or an infinity gets the scale NaN and reads back as NaN throughout.  A row of zeros gets the scale 1.
+// or an infinity gets the scale NaN and reads back as NaN throughout.  A row of zeros gets the scale 1 (K) or KV_ZERO_V.
 // A CTA takes TOK tokens: a warp each looks its sequence, position and page up, then every token's vectors
 // are dealt to 16 / TOK half-warps, each with its token's rotation row and the norm weights in registers and
 // four vectors' loads in flight.  Bound: HBM for many tokens (each row is read once and written once; TOK = 4
@@ -321,7 +327,7 @@ __global__ void __launch_bounds__(256, sizeof(TI) == 4 ? 3 : 4) kv_write_kernel(
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(mask, amax, o));
             float sc = amax * (1.f / 127.f);
-            if (sc == 0.f) sc = 1.f;
+            if (sc == 0.f) sc = is_v ? KV_ZERO_V : 1.f;
             uint32_t c[8];
             if (sc > 1e-30f) {  // x times the reciprocal is within 2^-15 of a step; 1.5 x 2^23 rounds it into the low byte
                 const float inv = __fdividef(1.0f, sc);

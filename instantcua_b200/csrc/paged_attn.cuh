@@ -17,10 +17,11 @@
 //   shared memory.  Rows behind the sequence's end are never read: cp.async fills zeros, so whatever a
 //   page still holds there (NaN included) cannot reach a sum.
 // * q8 rows are converted in registers, exactly: code -> 16-bit float by placing the byte in the
-//   mantissa of 1024 (fp16) or 128 / 256 (bf16) and subtracting.  The scales never round anything: the
+//   mantissa of 1024 (fp16) or 128 / 256 (bf16) and subtracting.  The scales add no rounding of their own: the
 //   K scale multiplies the fp32 score; the V scale enters the exponent, p' = 2^(s + log2 vs - m') with
 //   m' the running maximum of that sum, so the 16-bit operand of the P V product lies in [0, 256] whatever
-//   the scales are, and the row sum is l = sum p' / vs.
+//   the scales are, and the row sum is l = sum p' / vs.  (In fp16 a p' below 2^-14 is a subnormal number, off by
+//   up to 2^-25: less than that much of the largest |v| that counts.)
 // The running maximum is only moved (and the output rescaled) when a score exceeds it by more than 2^8: the
 // rescale is then rare, and p below 256 is as precise in 16 bits as p below 1.
 // Scores, maxima, sums and outputs are fp32; p is rounded once to the 16-bit type of q.

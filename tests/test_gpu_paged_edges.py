@@ -40,3 +40,26 @@ def test_halves_of_a_tile_without_a_position(n, kv, cache, typ):
         c.attend(same, same)
         assert torch.equal(same, first)
     assert c.flags() == 0
+
+
+@pytest.mark.parametrize("typ", [F16, BF16], ids=name)
+@pytest.mark.parametrize("size", [1e-5, 1e-4, 1e3])
+@pytest.mark.parametrize("n", [1, 3, 9, 90])
+def test_zero_v_rows_among_others(n, size, typ):
+    """Rows of zeros in V, as icua_kv_write leaves them in a q8 cache, among rows of one small (or large) size: they count in
+    the sum and hide nothing.  Every third key has one, the first and the last among them."""
+    total = n + 63
+    c = Cache([total], [total], cache="q8", typ=typ, n_kv=2, n_q=8)
+    qkv = c.randn(total, 12, 128)
+    qkv[:, 10:] = (1 + 0.1 * qkv[:, 10:]) * size
+    qkv[::3, 10:] = 0
+    qkv[-1, 10:] = 0
+    c.write(qkv.view(total, -1), None)
+    assert (c.read(F32)[1][::3] == 0).all()
+    c.n, c.total = [n], n
+    c.cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    q = c.randn(n, 8, 128).to(typ)
+    out = c.attend(q)
+    want, bound = c.attend64(q)
+    check_close(out, want, bound)
+    assert c.flags() == 0
