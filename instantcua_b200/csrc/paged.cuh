@@ -45,6 +45,13 @@ __device__ __forceinline__ SeqInfo load_seq(const SeqsView& S, int ps_shift, int
     return SeqInfo{q0, q1 - q0, kv};
 }
 
+// Raises ERR_SEQ if any sequence's entry contradicts itself; one warp.
+__device__ __forceinline__ void check_seqs(const SeqsView& S, int ps_shift, int lane, int* err) {
+    if (err == nullptr) return;
+#pragma unroll 4  // (the loads of four rounds in flight)
+    for (int s = lane; s < S.n_seqs; s += 32) load_seq(S, ps_shift, s, err);
+}
+
 // First pool row of position pos (any position of one page) of head h in sequence s, or -1 for a
 // table entry that names no page.
 __device__ __forceinline__ long long page_row(const PagesView& P, const SeqsView& S, int s, int h, int pos, int* err) {

@@ -191,11 +191,11 @@ struct PcTile {
 // The y-th tile of the batch, found by one warp: the last tile of every sequence (they see the most keys), then
 // the last but one of each, and so on, 32 sequences at a time; CTAs start in this order, so the long ones do
 // first.  False past the last one.
-__device__ __forceinline__ bool pc_find(const SeqsView& S, int ps_shift, int G, int min_rows, int y, int lane, PcTile& t, int* err) {
+__device__ __forceinline__ bool pc_find(const SeqsView& S, int ps_shift, int G, int min_rows, int y, int lane, PcTile& t) {
     int before = 0;
     for (int s0 = 0; s0 < S.n_seqs; s0 += 32) {
         SeqInfo q{0, 0, 0};
-        if (s0 + lane < S.n_seqs) q = load_seq(S, ps_shift, s0 + lane, err);
+        if (s0 + lane < S.n_seqs) q = load_seq(S, ps_shift, s0 + lane, nullptr);
         const int rows = q.n * G;
         const int tiles = rows > min_rows ? (rows + PC_ROWS - 1) / PC_ROWS : 0;
         const int all = __reduce_add_sync(0xffffffffu, tiles);
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
 
     if (warp == 0) {
         PcTile t{};
-        const bool live = pc_find(p.seqs, ps_shift, G, p.min_rows, y, lane, t, blockIdx.x == 0 ? p.err : nullptr);
+        const bool live = pc_find(p.seqs, ps_shift, G, p.min_rows, y, lane, t);
         if (live) pc_share(t, G, split, p.n_split);
         if (lane == 0) {
             tile_s = t;
@@ -263,6 +263,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
     } else if (warp == 8) {
         tmem_alloc(&tmem_slot, PC_TMEM_COLS);
         tmem_relinquish();
+    } else if (warp == 2 && blockIdx.x == 0) {  // (the tile search ends at the tile, not at the last sequence)
+        check_seqs(p.seqs, ps_shift, lane, p.err);
     } else if (threadIdx.x == 32) {
         mbar_init(q_full, 128);
         for (int i = 0; i < 2; ++i) {
@@ -732,7 +734,7 @@ __global__ void __launch_bounds__(256) paged_attn_tc_join_kernel(const PagedTcPa
     const int n_kv = p.pages.n_kv, G = p.group;
     const int r0 = (blockIdx.x & 7) * 32, h = (blockIdx.x >> 3) % n_kv, y = (blockIdx.x >> 3) / n_kv;
     PcTile t{};
-    const bool live = pc_find(p.seqs, p.pages.ps_shift, G, p.min_rows, y, lane, t, nullptr);
+    const bool live = pc_find(p.seqs, p.pages.ps_shift, G, p.min_rows, y, lane, t);
     if (!live || t.row0 + r0 >= t.n * G) return;
     pdl_wait();
     const float* pt0 = p.part + (size_t)(h + n_kv * p.n_split * y) * PC_PART + r0 + lane;

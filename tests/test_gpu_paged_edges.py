@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from _paged import Cache, check_close
+from instantcua_b200 import _lib as L
 
 pytestmark = pytest.mark.gpu
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
@@ -63,3 +64,27 @@ def test_zero_v_rows_among_others(n, size, typ):
     want, bound = c.attend64(q)
     check_close(out, want, bound)
     assert c.flags() == 0
+
+
+@pytest.mark.parametrize("change", ["length", "offset"])
+@pytest.mark.parametrize("n", [[40] * 40, [20] * 600, [300] + [1] * 70], ids=lambda n: f"{len(n)}")
+def test_attention_flags_contradictions_anywhere_in_a_batch(n, change):
+    """A sequence far behind the first 32 of a batch that contradicts itself is flagged and left alone, whichever kernels the
+    batch goes through."""
+    kv = [x + 10 for x in n]
+    c = Cache(n, kv, n_kv=2, n_q=4).fill()
+    q = c.randn(c.total, 4, 128).half()
+    clean = c.attend(q).clone()
+    assert c.flags() == 0
+    if change == "length":
+        s = len(n) - 5
+        c.kv_len[s] = -5
+        gone = slice(sum(n[:s]), sum(n[:s + 1]))
+    else:
+        c.cu[len(n)] = c.total + 1
+        gone = slice(c.total - n[-1], c.total)
+    out = c.attend(q, torch.full_like(q, 7))
+    assert c.flags() == L.FLAG_SEQ
+    assert (out[gone] == 7).all()
+    out[gone] = clean[gone]
+    assert torch.equal(out, clean)
