@@ -238,6 +238,8 @@ __global__ void __launch_bounds__(256, sizeof(TI) == 4 ? 3 : 4) kv_write_kernel(
             }
             tok_s[warp] = k;
         }
+    } else if (warp == 7 && blockIdx.x == 0) {  // (sequences whose rows no token looks up are checked too)
+        check_seqs(p.seqs, p.pages.ps_shift, lane, p.err);
     }
     __syncthreads();
     const int hw = threadIdx.x >> 4;
@@ -377,6 +379,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const KvReadParams p) {
     const int lane = threadIdx.x & 31, l = lane & 15;
     const long long unit = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;
     const int t = (int)(unit / p.n_groups), v0 = (int)(unit % p.n_groups) * VPT;
+    if (blockIdx.x == 0 && threadIdx.x >= 224) check_seqs(p.seqs, p.pages.ps_shift, lane, p.err);
     const int ta = __shfl_sync(0xffffffffu, t, 0), tb = __shfl_sync(0xffffffffu, t, 16);
     const int sa = find_seq(p.seqs, ta, lane);
     const int sb = tb == ta ? sa : find_seq(p.seqs, tb, lane);

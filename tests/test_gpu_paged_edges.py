@@ -88,3 +88,39 @@ def test_attention_flags_contradictions_anywhere_in_a_batch(n, change):
     assert (out[gone] == 7).all()
     out[gone] = clean[gone]
     assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("cache", [F16, "q8"], ids=name)
+@pytest.mark.parametrize("seqs", [3, 80])
+@pytest.mark.parametrize("length", [-1, 1 << 29])
+def test_write_and_read_flag_idle_sequences_that_contradict_themselves(seqs, length, cache):
+    """An idle sequence with an impossible length: no token looks it up, the flag is set all the same, and the other
+    sequences' rows are written and read."""
+    n = [1] * seqs
+    n[seqs - 2] = 0
+    c = Cache(n, [9] * seqs, cache=cache, junk=2.0).fill()
+    qkv = c.randn(c.total, 8 * 128)
+    c.write(qkv, None)
+    clean = c.read(F16)
+    assert c.flags() == 0
+    c.kv_len[seqs - 2] = length
+    got = c.read(F16)
+    assert c.flags() == L.FLAG_SEQ
+    assert torch.equal(got[0], clean[0]) and torch.equal(got[1], clean[1])
+    c.err.zero_()
+    c.fill()
+    c.write(qkv, None)
+    assert c.flags() == L.FLAG_SEQ
+    got = c.read(F16)
+    assert torch.equal(got[0], clean[0]) and torch.equal(got[1], clean[1])
+
+
+def test_write_and_read_flag_offsets_that_no_token_meets():
+    """cu_q = 0, 4, 2, 2, 6: sequence 1 descends, and no row's lookup ends at it."""
+    c = Cache([2, 0, 0, 4], [20] * 4, junk=2.0).fill()
+    c.cu.copy_(torch.tensor([0, 4, 2, 2, 6]))
+    c.write(c.randn(6, 8 * 128), None)
+    assert c.flags() == L.FLAG_SEQ
+    c.err.zero_()
+    c.read(F16)
+    assert c.flags() == L.FLAG_SEQ
