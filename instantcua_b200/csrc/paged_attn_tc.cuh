@@ -735,8 +735,8 @@ __global__ void __launch_bounds__(256) paged_attn_tc_join_kernel(const PagedTcPa
     const int r0 = (blockIdx.x & 7) * 32, h = (blockIdx.x >> 3) % n_kv, y = (blockIdx.x >> 3) / n_kv;
     PcTile t{};
     const bool live = pc_find(p.seqs, p.pages.ps_shift, G, p.min_rows, y, lane, t);
+    pdl_wait();  // (every CTA: what follows in the stream relies on this grid not being done before the one it joins)
     if (!live || t.row0 + r0 >= t.n * G) return;
-    pdl_wait();
     const float* pt0 = p.part + (size_t)(h + n_kv * p.n_split * y) * PC_PART + r0 + lane;
     float m = -INFINITY, l = 0.f;
     float4 a[4];

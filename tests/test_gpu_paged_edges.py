@@ -124,3 +124,28 @@ def test_write_and_read_flag_offsets_that_no_token_meets():
     c.err.zero_()
     c.read(F16)
     assert c.flags() == L.FLAG_SEQ
+
+
+@pytest.mark.parametrize("cache,typ", TYPES, ids=name)
+def test_more_tokens_promised_than_any_sequence_has(cache, typ):
+    """max_q far above every sequence's tokens: the tensor-core kernel and its join find nothing to do.  Calls that follow one
+    another in the stream with other offsets each attend their own batch, and flag their own contradictions."""
+    n, kv = [1, 3, 2, 0], [3000, 700, 40, 9]
+    c = Cache(n, kv, cache=cache, typ=typ, n_kv=2, n_q=8).fill()
+    q = (c.randn(c.total, 8, 128) * 2).to(typ)
+    want, bound = c.attend64(q)
+    good, idle, bad = c.cu.clone(), torch.zeros_like(c.cu), c.kv_len.clone()
+    bad[3] = -7
+    sc = c.scratch(max_q=500)
+    for _ in range(20):
+        c.cu.copy_(good)
+        out = c.attend(q, torch.full_like(q, 5.0), max_q=500, scratch=sc)
+        c.cu.copy_(idle)
+        none = c.attend(q, torch.full_like(q, 5.0), max_q=500, scratch=sc)
+        assert (none == 5).all()
+        check_close(out, want, bound)
+    assert c.flags() == 0
+    c.cu.copy_(good)
+    c.kv_len.copy_(bad)
+    check_close(c.attend(q, max_q=500, scratch=sc), want, bound)
+    assert c.flags() == L.FLAG_SEQ
