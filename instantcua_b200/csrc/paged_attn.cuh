@@ -162,7 +162,11 @@ __device__ __forceinline__ PaWork pa_work(const SeqsView& S, int ps_shift, int n
     return w;
 }
 
-// pre[s] = units before sequence s, pre[n_seqs] = all of them.  `warp_tot` holds one word per warp.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return a + b < a ? 0xffffffffu : a + b; }
+
+// pre[s] = units before sequence s, pre[n_seqs] = all of them.  `warp_tot` holds one word per warp.  Offsets that
+// contradict each other can claim the same rows many times over, so that the units pass 32 bits although the call's
+// check of its sizes holds: the sums stop at the largest word, and such a batch counts as one without tokens.
 template <int THREADS>
 __device__ __forceinline__ uint32_t pa_prefix(const SeqsView& S, int ps_shift, int n_kv, int group, int max_rows, int tile_rows,
                                               int block, uint32_t* pre, uint32_t* warp_tot, int* err, bool alone = false) {
@@ -173,13 +177,13 @@ __device__ __forceinline__ uint32_t pa_prefix(const SeqsView& S, int ps_shift, i
         uint32_t w = 0;
         if (s < S.n_seqs) {
             const PaWork k = pa_work(S, ps_shift, n_kv, group, max_rows, tile_rows, block, s, err, alone);
-            w = (uint32_t)k.items * (uint32_t)k.units();
+            w = (uint32_t)min((unsigned long long)k.items * (unsigned long long)k.units(), 0xffffffffull);
         }
         uint32_t x = w;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
+            if (lane >= o) x = add_sat(x, y);
         }
         if (lane == 31) warp_tot[warp] = x;
         __syncthreads();
@@ -187,11 +191,15 @@ __device__ __forceinline__ uint32_t pa_prefix(const SeqsView& S, int ps_shift, i
 #pragma unroll
         for (int i = 0; i < THREADS / 32; ++i) {
             if (i < warp) before += warp_tot[i];
-            all += warp_tot[i];
+            all = add_sat(all, warp_tot[i]);
         }
         if (s < S.n_seqs) pre[s] = before + x - w;
-        base += all;
+        base = add_sat(base, all);
         __syncthreads();
+    }
+    if (base == 0xffffffffu) {
+        if (tid == 0 && err) atomicOr(err, ERR_SEQ);
+        return 0;
     }
     if (tid == 0) pre[S.n_seqs] = base;
     __syncthreads();

@@ -149,3 +149,20 @@ def test_more_tokens_promised_than_any_sequence_has(cache, typ):
     c.kv_len.copy_(bad)
     check_close(c.attend(q, max_q=500, scratch=sc), want, bound)
     assert c.flags() == L.FLAG_SEQ
+
+
+def test_offsets_that_claim_rows_over_and_over():
+    """Descending offsets under which 683 of 1,024 sequences claim the same 64 rows, over nearly two million positions each,
+    with more rows a sequence than max_q says: 683 x 2 tiles x 128 heads x 30,360 blocks pass 32 bits.  Nothing is followed
+    or written, the flag is set."""
+    c = Cache([1], [5], n_kv=128, n_q=128)
+    pages, q = 7590, c.randn(64, 128, 128).half()
+    c.ps, c.n_pages, c.total, c.max_pages = 256, 1, 64, pages
+    c.k, c.v = (torch.zeros(128 * 256, 128, device="cuda", dtype=F16) for _ in range(2))
+    c.cu = torch.tensor([0, 32, 64] * 341 + [0, 32], dtype=torch.int32, device="cuda")
+    c.kv_len = torch.full((1024,), pages * 256, dtype=torch.int32, device="cuda")
+    c.table = torch.full((1024, pages), -1, dtype=torch.int32, device="cuda")
+    assert int((c.cu[1:] > c.cu[:-1]).sum()) * 2 * 128 * (pages * 256 // 64) > 2**32
+    out = c.attend(q, torch.full_like(q, 7.0), n_seqs=1024, max_q=16, max_kv=pages * 256)
+    assert c.flags() == L.FLAG_SEQ
+    assert (out == 7).all()
