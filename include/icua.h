@@ -405,7 +405,9 @@ typedef struct icua_attn_paged_args {
     uint64_t scratch_bytes;    /*   overlap in time need one each */
 } icua_attn_paged_args;
 /* Bytes of scratch that icua_attn_paged needs for these sizes (n_seqs, total_q, max_q; the arrays are
- * not read); 0 for arguments that it would refuse. */
+ * not read); 0 for arguments that it would refuse.  Refused as too large: total_q * n_q / n_kv above
+ * 2^31 - 1, and tables so wide that the blocks of keys of all sequences and heads could pass 32 bits
+ * (never below n_seqs * n_kv * max_pages * page_size = 10^11). */
 uint64_t icua_attn_paged_scratch_bytes(const icua_kv_pages* pages, const icua_kv_seqs* seqs, int32_t n_q);
 /* Causal attention of every new token over its sequence's cache up to its own position (which
  * icua_kv_write has filled): one token per sequence (decode), drafts, chunks of a prompt and whole

@@ -267,9 +267,11 @@ icua_status check_attn(const icua_kv_pages* pages, const icua_kv_seqs* seqs, int
     const icua_status st = check_cache(pages, seqs, P, S);
     if (st != ICUA_OK) return st;
     if (n_q < pages->n_kv || n_q > 256 || n_q % pages->n_kv) return bad("n_q %d is not a multiple of n_kv %d up to 256", n_q, pages->n_kv);
-    // the kernels count blocks of keys over all items in 32 bits
+    // rows are counted in 32 bits, and so are the few-rows kernel's blocks of keys over all its items: tiles of sixteen rows
+    // at least, of sequences with PA_ROWS_FEW rows at most
     const int64_t rows = (int64_t)seqs->total_q * (n_q / pages->n_kv);
-    const double blocks = ((double)rows / 16 + seqs->n_seqs) * pages->n_kv * ((double)seqs->max_pages * pages->page_size / 64 + 1 + PA_ITEM);
+    const double tiles = std::min((double)rows / 16 + seqs->n_seqs, (PA_ROWS_FEW / 16.0) * seqs->n_seqs);
+    const double blocks = tiles * pages->n_kv * ((double)seqs->max_pages * pages->page_size / 64 + 1 + PA_ITEM);
     if (rows > INT32_MAX || blocks > 4e9) return bad("the batch is too large: split it");
     return ICUA_OK;
 }

@@ -107,3 +107,22 @@ def test_empty_batches_are_no_work():
         assert lib.icua_kv_write(p, C.byref(s), C.byref(rows()), None, None) == L.OK
         assert lib.icua_kv_read(p, C.byref(s), A, A, L.DT_F32, None, None) == L.OK
         assert lib.icua_attn_paged(p, C.byref(s), C.byref(attn()), None, None) == L.OK
+
+
+@pytest.mark.parametrize("total_q,n_q", [(32768, 128), (65536, 64), (1 << 20, 64)])
+def test_long_prompts_with_wide_tables_are_taken(total_q, n_q):
+    """The size limit counts rows of short sequences only: whole prompts beside a page table for a million positions."""
+    p = pages(n_kv=8, page_size=256)
+    s = seqs(n_seqs=1, total_q=total_q, max_q=total_q, max_kv=total_q, max_pages=4096)
+    assert L.lib().icua_attn_paged_scratch_bytes(C.byref(p), C.byref(s), n_q) > 0
+
+
+def test_batches_past_the_counters_are_refused():
+    p = C.byref(pages(n_kv=128, page_size=256))
+    for s in (seqs(n_seqs=1024, total_q=1024, max_pages=1 << 22),   # 1,024 x 128 items over 2^30 positions
+              seqs(n_seqs=1, total_q=1 << 25, max_q=1 << 25)):      # 2^25 tokens x 64 heads a kv head
+        n_q = 128 if s.n_seqs > 1 else 256
+        if s.n_seqs == 1:
+            p = C.byref(pages(n_kv=4))
+        assert L.lib().icua_attn_paged_scratch_bytes(p, C.byref(s), n_q) == 0
+        refused(L.lib().icua_attn_paged(p, C.byref(s), C.byref(attn(n_q=n_q)), None, None))

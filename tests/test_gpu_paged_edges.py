@@ -166,3 +166,13 @@ def test_offsets_that_claim_rows_over_and_over():
     out = c.attend(q, torch.full_like(q, 7.0), n_seqs=1024, max_q=16, max_kv=pages * 256)
     assert c.flags() == L.FLAG_SEQ
     assert (out == 7).all()
+
+
+def test_a_chunk_beside_a_table_for_a_million_positions():
+    """40 tokens of 128 heads over 8 kv heads with a page table of 2^20 positions, in a batch padded to 32,768 rows."""
+    c = Cache([40], [300], n_kv=8, n_q=128, ps=256, pad=32728, max_pages=4096).fill()
+    q = c.randn(c.total, 128, 128).half()
+    out = c.attend(q, max_q=c.total)
+    want, bound = c.attend64(q)
+    check_close(out[:40], want[:40], bound[:40])
+    assert c.flags() == 0
