@@ -247,7 +247,7 @@ TcGrid tc_grid(const icua_kv_seqs* s, int n_kv, int group, int min_rows, int n_s
     TcGrid g;
     g.tiles = (int)(rows / PC_ROWS + std::min<int64_t>(s->n_seqs, rows / (min_rows + 1)));
     const int base = g.tiles * n_kv;
-    g.n_split = std::max(1, std::min(std::min(n_sm, PC_MAX_SHARES) / std::max(base, 1), (s->max_kv + 2 * PC_BK - 1) / (2 * PC_BK)));
+    g.n_split = std::max(1, std::min(std::min(n_sm, PC_MAX_SHARES) / std::max(base, 1), (int)(((int64_t)s->max_kv + 2 * PC_BK - 1) / (2 * PC_BK))));
     return g;
 }
 

@@ -176,3 +176,13 @@ def test_a_chunk_beside_a_table_for_a_million_positions():
     want, bound = c.attend64(q)
     check_close(out[:40], want[:40], bound[:40])
     assert c.flags() == 0
+
+
+@pytest.mark.parametrize("n,kv", [([200], [9000]), ([1, 60], [5000, 700]), ([1], [3000])], ids=str)
+def test_the_largest_length_hint(n, kv):
+    """max_kv up to 2^31 - 1 splits the keys as any other hint above all lengths does: the same bits."""
+    c = Cache(n, kv).fill()
+    q = c.randn(c.total, 4, 128).half()
+    want = c.attend(q, max_kv=1 << 20)
+    for hint in (2**31 - 256, 2**31 - 255, 2**31 - 1):
+        assert torch.equal(c.attend(q, max_kv=hint), want)
