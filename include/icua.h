@@ -400,7 +400,7 @@ typedef struct icua_attn_paged_args {
     int64_t q_stride, out_stride; /* elements between two tokens, multiples of 8; 0 = n_q * 128 */
     int32_t dtype;             /* of q and out: ICUA_DT_BF16 or ICUA_DT_F16; the cache's type where that is 16-bit */
     int32_t n_q;               /* query heads, a multiple of n_kv; head h reads kv head h / (n_q / n_kv) */
-    float scale;               /* of the scores; 0 = 1 / sqrt(128) */
+    float scale;               /* of the scores, up to 2.3e38 (times log2(e) it stays finite); 0 = 1 / sqrt(128) */
     void* scratch;             /* device memory for parts of rows, no initialisation needed; calls that can */
     uint64_t scratch_bytes;    /*   overlap in time need one each */
 } icua_attn_paged_args;

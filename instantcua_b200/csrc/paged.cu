@@ -2,6 +2,7 @@
 // variant and launch.  Kernels: paged.cuh (write, read back), paged_attn.cuh and paged_attn_tc.cuh
 // (attention of few and of many rows).
 #include <algorithm>
+#include <cfloat>
 #include <cstdarg>
 #include <cstdio>
 #include <type_traits>
@@ -363,7 +364,8 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
     p.out_stride = a->out_stride ? a->out_stride : (int64_t)a->n_q * HD;
     if (p.q_stride < (int64_t)a->n_q * HD || p.q_stride % 8 || p.out_stride < (int64_t)a->n_q * HD || p.out_stride % 8)
         return bad("token strides are multiples of 8, at least a row (or 0)");
-    if (!(a->scale >= 0.f) || a->scale > 3e38f) return bad("scale is negative or not finite");
+    p.scale_log2 = (a->scale > 0.f ? a->scale : 0.08838834764831845f) * 1.4426950408889634f;  // (scores in units of log2)
+    if (!(a->scale >= 0.f) || !(p.scale_log2 <= FLT_MAX)) return bad("scale is negative or, in units of log2, not finite");
     if (!a->scratch || !aligned(a->scratch, 16) || a->scratch_bytes < icua_attn_paged_scratch_bytes(pages, seqs, a->n_q))
         return bad("scratch is null, not 16-byte aligned or smaller than icua_attn_paged_scratch_bytes");
     if (seqs->n_seqs == 0 || seqs->total_q == 0) return ICUA_OK;
@@ -373,7 +375,6 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
     p.out = a->out;
     p.n_q = a->n_q;
     p.group = a->n_q / pages->n_kv;
-    p.scale_log2 = (a->scale > 0.f ? a->scale : 0.08838834764831845f) * 1.4426950408889634f;
     p.max_rows = PA_ROWS_FEW;
     p.part = (float*)a->scratch;
     p.split = (PaSplit*)(p.part + (size_t)PA_MAX_CTAS * 2 * PA_PART);

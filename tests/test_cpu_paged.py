@@ -126,3 +126,10 @@ def test_batches_past_the_counters_are_refused():
             p = C.byref(pages(n_kv=4))
         assert L.lib().icua_attn_paged_scratch_bytes(p, C.byref(s), n_q) == 0
         refused(L.lib().icua_attn_paged(p, C.byref(s), C.byref(attn(n_q=n_q)), None, None))
+
+
+def test_scale_stays_finite_in_units_of_log2():
+    """scale * log2(e) passes fp32's largest number from 2.36e38 on: scores of 0 would turn into NaN."""
+    for scale in (2.4e38, 2.9e38):
+        refused(L.lib().icua_attn_paged(C.byref(pages()), C.byref(seqs()), C.byref(attn(scale=scale)), None, None))
+    assert L.lib().icua_attn_paged(C.byref(pages()), C.byref(seqs(n_seqs=0)), C.byref(attn(scale=2.3e38)), None, None) == L.OK
