@@ -396,7 +396,7 @@ icua_status icua_kv_read(const icua_kv_pages* pages, const icua_kv_seqs* seqs, v
 
 typedef struct icua_attn_paged_args {
     const void* q;             /* [total_q][n_q][128] */
-    void* out;                 /* the same shape; may be q itself */
+    void* out;                 /* the same shape; may be q itself, with q's stride, and overlaps it in no other way */
     int64_t q_stride, out_stride; /* elements between two tokens, multiples of 8; 0 = n_q * 128 */
     int32_t dtype;             /* of q and out: ICUA_DT_BF16 or ICUA_DT_F16; the cache's type where that is 16-bit */
     int32_t n_q;               /* query heads, a multiple of n_kv; head h reads kv head h / (n_q / n_kv) */

@@ -364,6 +364,8 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
     p.out_stride = a->out_stride ? a->out_stride : (int64_t)a->n_q * HD;
     if (p.q_stride < (int64_t)a->n_q * HD || p.q_stride % 8 || p.out_stride < (int64_t)a->n_q * HD || p.out_stride % 8)
         return bad("token strides are multiples of 8, at least a row (or 0)");
+    // (a row written at its place in out would be another token's q)
+    if (a->q == a->out && p.q_stride != p.out_stride && seqs->total_q > 1) return bad("out is q itself, with another token stride");
     p.scale_log2 = (a->scale > 0.f ? a->scale : 0.08838834764831845f) * 1.4426950408889634f;  // (scores in units of log2)
     if (!(a->scale >= 0.f) || !(p.scale_log2 <= FLT_MAX)) return bad("scale is negative or, in units of log2, not finite");
     if (!a->scratch || !aligned(a->scratch, 16) || a->scratch_bytes < icua_attn_paged_scratch_bytes(pages, seqs, a->n_q))

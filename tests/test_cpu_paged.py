@@ -133,3 +133,12 @@ def test_scale_stays_finite_in_units_of_log2():
     for scale in (2.4e38, 2.9e38):
         refused(L.lib().icua_attn_paged(C.byref(pages()), C.byref(seqs()), C.byref(attn(scale=scale)), None, None))
     assert L.lib().icua_attn_paged(C.byref(pages()), C.byref(seqs(n_seqs=0)), C.byref(attn(scale=2.3e38)), None, None) == L.OK
+
+
+def test_in_place_attention_keeps_the_stride():
+    """out = q with another token stride would write over rows of q that are still to be read."""
+    lib, p = L.lib(), C.byref(pages())
+    for kw in (dict(q_stride=520), dict(out_stride=1024), dict(q_stride=1024, out_stride=520)):
+        refused(lib.icua_attn_paged(p, C.byref(seqs()), C.byref(attn(**kw)), None, None))
+    for kw in (dict(), dict(q_stride=520, out_stride=520), dict(q_stride=512), dict(out_stride=520, out=2 * A)):
+        assert lib.icua_attn_paged(p, C.byref(seqs(n_seqs=0)), C.byref(attn(**kw)), None, None) == L.OK
