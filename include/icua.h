@@ -306,7 +306,9 @@ icua_status icua_greedy_head_noalloc(int32_t vocab, const void* packed_embed_dev
  * on the current device (default 4194304).  No reference counterpart: it exists so that tests can
  * make that wait give up (polls = 0) and check the timeout report -- the kernel flags the step,
  * still waits for its copy with the default bound, the engine call returns ICUA_ERR_TIMEOUT and
- * later calls on that engine ICUA_ERR_STATE.  Set it back before running other work. */
+ * later calls on that engine ICUA_ERR_STATE.  Also the limit of the last wait of icua_attn_paged's
+ * tensor-core kernel, in the calls made from then on (on any device): its rows become NaN and it raises
+ * ICUA_FLAG_WAIT.  Set it back before running other work. */
 icua_status icua_set_wait_limit(uint32_t polls);
 
 /* Bit-exact dequantization of a packed device matrix to fp32 row-major [n_rows, k]. */
@@ -327,7 +329,9 @@ icua_status icua_dequant(int32_t fmt, int32_t n_rows, int32_t k, const void* pac
  * positions masked) and sets ICUA_FLAG_PAGE; a sequence whose entries contradict each other (cu_q
  * that descends or passes total_q, a length below 0 or above max_pages * page_size) counts as
  * without tokens, a token without a position or a rotation row is left out, and both set
- * ICUA_FLAG_SEQ.  err_dev: optional device int32 that the flags are OR-ed into. */
+ * ICUA_FLAG_SEQ.  ICUA_FLAG_WAIT: a bounded wait inside icua_attn_paged gave up; the rows it was for
+ * are NaN.  err_dev: optional device int32 that the flags are OR-ed into; without it left-out tokens
+ * show by their rows alone. */
 enum { ICUA_DT_F32 = 0, ICUA_DT_BF16 = 1, ICUA_DT_F16 = 2 }; /* row types, as icua_gemv's x_dtype */
 /* Third cache type: int8 codes with one fp32 scale per row (position, head): scale = max|x| / 127,
  * code = x / scale to the nearest (2^-15 of a step around a tie may go either way); a row of zeros has

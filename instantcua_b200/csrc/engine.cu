@@ -14,6 +14,7 @@
 #include <unistd.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 #include <chrono>
 #include <cmath>
@@ -218,6 +219,7 @@ icua_status set_global_error(icua_status s, const char* msg) {
     g_error = msg;
     return s;
 }
+extern std::atomic<uint32_t> paged_wait_polls;
 }  // namespace icua_host
 
 namespace {
@@ -2810,6 +2812,7 @@ icua_status icua_set_wait_limit(uint32_t polls) {
     icua_engine* eng = nullptr;
     CK(cudaMemcpyToSymbol(c_norm_wait_polls, &polls, sizeof polls));
     CK(cudaDeviceSynchronize());
+    icua_host::paged_wait_polls.store(polls, std::memory_order_relaxed);
     return ICUA_OK;
 }
 

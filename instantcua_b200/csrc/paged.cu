@@ -2,6 +2,7 @@
 // variant and launch.  Kernels: paged.cuh (write, read back), paged_attn.cuh and paged_attn_tc.cuh
 // (attention of few and of many rows).
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <cstdarg>
 #include <cstdio>
@@ -14,6 +15,7 @@
 
 namespace icua_host {
 icua_status set_global_error(icua_status s, const char* msg);
+std::atomic<uint32_t> paged_wait_polls{1u << 22};  // icua_set_wait_limit
 }
 
 using namespace icua;
@@ -404,6 +406,7 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
         c.err = err_dev;
         const TcGrid g = tc_grid(seqs, pages->n_kv, p.group, c.min_rows, sm_count(dev));
         c.n_split = g.n_split;
+        c.polls = icua_host::paged_wait_polls.load(std::memory_order_relaxed);
         tc_ran = g.tiles > 0;
         if (tc_ran)
             e = q8 ? (f16 ? launch_attn_tc<__half, true>(c, g.tiles, dev, s) : launch_attn_tc<__nv_bfloat16, true>(c, g.tiles, dev, s))

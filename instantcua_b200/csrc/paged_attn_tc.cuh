@@ -23,8 +23,8 @@
 // 500 over 8,001 positions, 16:8 heads, q8, 84 us, there bound by the four converting warps (1,800 clocks per
 // 128 rows) and by the factors' shared-memory reads.  Tried and slower: part of the exponentials as polynomials
 // on the FMA pipe (560 against 549 us), two threads per row (575), rows as matrix fragments (608).
-// Every wait is bounded: one that gives up raises ERR_WAIT_PREFILL and the CTA still drains its copies
-// and products and frees its tensor memory.
+// Every wait is bounded: one that gives up raises ERR_WAIT_PREFILL, the half's rows become NaN, and the CTA still
+// drains its copies and products and frees its tensor memory.
 #pragma once
 #include "paged_attn.cuh"
 
@@ -75,6 +75,7 @@ struct PagedTcParams {
     float scale_log2;
     int min_rows;  // sequences with at most so many rows belong to the other kernel
     int n_split;
+    uint32_t polls;  // limit of the last wait of a half's softmax
     float* part;   // [gridDim.x][PC_PART] when n_split > 1
     int* err;
 };
@@ -664,10 +665,18 @@ __global__ void __launch_bounds__(PC_THREADS, 1) paged_attn_tc_kernel(const Page
         }
         // The rows go out through the half's q tile: behind its last product or, where no row has a position and so no
         // product runs, behind the copies that fill the tile.
-        if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(nb > 0 ? &o_full[hf] : q_full, 0))) ok = false;
+        if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(nb > 0 ? &o_full[hf] : q_full, 0, p.polls))) ok = false;
         tc_fence_after();
         if (!ok) {
+            // rows that are lost are NaN, whether or not the caller reads flags
             if (lane == 0 && p.err) atomicOr(p.err, ERR_WAIT_PREFILL);
+            if (p.n_split > 1) {  // (the join keeps a NaN maximum)
+                float* pt = p.part + (size_t)blockIdx.x * PC_PART + PC_ROWS * HD + 128 * hf + 32 * quarter + lane;
+                pt[0] = pt[PC_ROWS] = __int_as_float(0x7fffffff);
+            } else if (R < rows) {
+                uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + (t.q0 + R / G) * p.out_stride + (h * G + R % G) * HD);
+                for (int c = 0; c < 16; ++c) dst[c] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+            }
         } else {
             const float sum = l.x + l.y;
             const int rt = 128 * hf + 32 * quarter + lane;  // row of the tile

@@ -186,3 +186,28 @@ def test_the_largest_length_hint(n, kv):
     want = c.attend(q, max_kv=1 << 20)
     for hint in (2**31 - 256, 2**31 - 255, 2**31 - 1):
         assert torch.equal(c.attend(q, max_kv=hint), want)
+
+
+@pytest.mark.parametrize("cache,typ", TYPES, ids=name)
+@pytest.mark.parametrize("n,kv", [([300], [300]), ([300], [9000]), ([200, 3, 1], [250, 40, 2000])], ids=str)
+def test_a_wait_that_gives_up_leaves_nan_rows_and_a_flag(n, kv, cache, typ):
+    """The tensor-core kernel's last wait with a limit of no polls: its rows become NaN (written at once, or through the join
+    of key shares), with and without a flag word; the others and the next call are as ever."""
+    c = Cache(n, kv, cache=cache, typ=typ, n_kv=2, n_q=8).fill()
+    q = (c.randn(c.total, 8, 128) * 2).to(typ)
+    want = c.attend(q).clone()
+    lib = L.lib()
+    try:
+        L.check(lib.icua_set_wait_limit(0))
+        lost = c.attend(q, torch.full_like(q, 7.0))
+        assert c.flags() == L.FLAG_WAIT
+        err, c.err = c.err, None
+        silent = c.attend(q, torch.full_like(q, 7.0))
+        c.err = err
+        torch.cuda.synchronize()
+    finally:
+        L.check(lib.icua_set_wait_limit(1 << 22))
+    for out in (lost, silent):
+        assert out[:n[0]].isnan().all() and torch.equal(out[n[0]:], want[n[0]:])
+    c.err.zero_()
+    assert torch.equal(c.attend(q), want) and c.flags() == 0
