@@ -324,7 +324,9 @@ icua_status icua_dequant(int32_t fmt, int32_t n_rows, int32_t k, const void* pac
  * (int32 arrays: 4).  The calls only launch on `stream` (a cudaStream_t or NULL): nothing is
  * allocated, copied or waited for, so they can be captured into a graph.  Lengths and page numbers
  * are read by the kernels, so a captured call follows what the arrays hold when it is replayed.
- * Arguments the host can see are checked before anything is launched.  What only the device can see
+ * Arguments the host can see are checked before anything is launched, and pointers to be memory of the
+ * current device (or managed memory; other than the pools and rows they may be pinned host memory, which
+ * is read in place), not how far it reaches.  What only the device can see
  * is checked there: a page number outside [0, n_pages) is left out (not written, read as zeros, its
  * positions masked) and sets ICUA_FLAG_PAGE; a sequence whose entries contradict each other (cu_q
  * that descends or passes total_q, a length below 0 or above max_pages * page_size) counts as

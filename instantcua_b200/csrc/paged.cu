@@ -6,6 +6,7 @@
 #include <cfloat>
 #include <cstdarg>
 #include <cstdio>
+#include <initializer_list>
 #include <type_traits>
 
 #include "../../include/icua.h"
@@ -39,14 +40,61 @@ icua_status cuda_fail(const char* what, cudaError_t e) {
 
 bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
-// A pointer that the kernels may follow: device (or managed) memory of the current device.
-icua_status check_device_ptr(const void* p, int dev, const char* name) {
-    cudaPointerAttributes a;
-    const cudaError_t e = cudaPointerGetAttributes(&a, p);
-    if (e != cudaSuccess) return cuda_fail("cudaPointerGetAttributes", e);
-    if (a.type == cudaMemoryTypeManaged) return ICUA_OK;
-    if (a.type != cudaMemoryTypeDevice) return bad("%s is not device memory", name);
-    if (a.device != dev) return bad("%s is on device %d, the current device is %d", name, a.device, dev);
+// cuPointerGetAttributes (about 50 ns a pointer; the runtime's call takes 70).
+using PointerAttributes = CUresult (*)(unsigned, CUpointer_attribute*, void**, CUdeviceptr);
+PointerAttributes pointer_attributes() {
+    static const PointerAttributes fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const cudaError_t e = cudaGetDriverEntryPoint("cuPointerGetAttributes", &f, cudaEnableDefault, &q);
+        return e == cudaSuccess && q == cudaDriverEntryPointSuccess ? (PointerAttributes)f : nullptr;
+    }();
+    return fn;
+}
+
+struct Named {
+    const void* p;  // NULL: not given
+    const char* name;
+};
+// Pointers that the kernels may follow: memory of the current device, or managed memory; the first two (a pool and a row
+// array) no host memory, the others also pinned host memory, which the device reads in place.
+icua_status check_device_ptrs(int* dev, std::initializer_list<Named> list) {
+    const cudaError_t e = cudaGetDevice(dev);
+    if (e != cudaSuccess) return cuda_fail("cudaGetDevice", e);
+    const PointerAttributes get = pointer_attributes();
+    if (!get) return cuda_fail("cuPointerGetAttributes", cudaErrorSymbolNotFound);
+    // (small arrays often share an allocation: a pointer into one that has been looked up is not looked up again)
+    struct Range {
+        CUdeviceptr begin;
+        size_t bytes;
+    } seen[16];
+    int i = 0, n_seen = 0;
+    for (const Named& n : list) {
+        const bool host = i++ >= 2;
+        if (!n.p) continue;
+        const CUdeviceptr p = (CUdeviceptr)n.p;
+        bool known = false;
+        for (int k = 0; k < n_seen; ++k) known |= p - seen[k].begin < seen[k].bytes;
+        if (known) continue;
+        unsigned type = 0;
+        int at = -1;
+        Range r{};
+        CUpointer_attribute what[4] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL,
+                                       CU_POINTER_ATTRIBUTE_RANGE_START_ADDR, CU_POINTER_ATTRIBUTE_RANGE_SIZE};
+        void* to[4] = {&type, &at, &r.begin, &r.bytes};
+        if (get(4, what, to, p) != CUDA_SUCCESS) type = 0;
+        if (type == CU_MEMORYTYPE_DEVICE && at == *dev) {
+            if (n_seen < 16) seen[n_seen++] = r;
+            continue;
+        }
+        if (type == CU_MEMORYTYPE_HOST && host) continue;
+        unsigned managed = 0;
+        what[0] = CU_POINTER_ATTRIBUTE_IS_MANAGED;
+        to[0] = &managed;
+        if (type != 0 && get(1, what, to, p) == CUDA_SUCCESS && managed) continue;
+        if (type != CU_MEMORYTYPE_DEVICE) return bad("%s is not device memory", n.name);
+        return bad("%s is on device %d, the current device is %d", n.name, at, *dev);
+    }
     return ICUA_OK;
 }
 
@@ -87,13 +135,6 @@ icua_status check_cache(const icua_kv_pages* c, const icua_kv_seqs* s, PagesView
     P->n_pages = c->n_pages;
     *S = SeqsView{s->cu_q, s->kv_len, s->page_table, s->n_seqs, s->total_q, s->max_pages};
     return ICUA_OK;
-}
-
-icua_status current(const icua_kv_pages* c, const void* rows, int* dev) {
-    const cudaError_t e = cudaGetDevice(dev);
-    if (e != cudaSuccess) return cuda_fail("cudaGetDevice", e);
-    icua_status st = check_device_ptr(c->k, *dev, "the K pool");
-    return st != ICUA_OK ? st : check_device_ptr(rows, *dev, "the row array");
 }
 
 constexpr int MAX_DEVICES = 64;
@@ -304,7 +345,13 @@ icua_status icua_kv_write(const icua_kv_pages* pages, const icua_kv_seqs* seqs, 
     if (!(rows->eps >= 0.f)) return bad("eps is negative or NaN");
     if (seqs->n_seqs == 0 || seqs->total_q == 0) return ICUA_OK;
     int dev = 0;
-    if ((st = current(pages, rows->qkv, &dev)) != ICUA_OK) return st;
+    const bool scales = pages->dtype == ICUA_KV_Q8;
+    st = check_device_ptrs(&dev, {{pages->k, "the K pool"}, {rows->qkv, "the row array"}, {pages->v, "the V pool"},
+                                 {scales ? pages->k_scale : nullptr, "k_scale"}, {scales ? pages->v_scale : nullptr, "v_scale"},
+                                 {seqs->cu_q, "cu_q"}, {seqs->kv_len, "kv_len"}, {seqs->page_table, "page_table"}, {err_dev, "err_dev"},
+                                 {rows->q_norm, "q_norm"}, {rows->k_norm, "k_norm"}, {rows->rope, "rope"},
+                                 {rows->rope ? rows->rope_rows : nullptr, "rope_rows"}, {rows->q_out, "q_out"}});
+    if (st != ICUA_OK) return st;
     p.qkv = rows->qkv;
     p.q_norm = rows->q_norm;
     p.k_norm = rows->k_norm;
@@ -334,7 +381,12 @@ icua_status icua_kv_read(const icua_kv_pages* pages, const icua_kv_seqs* seqs, v
     if ((int64_t)seqs->total_q * 2 * pages->n_kv > ((int64_t)16 << 31) - 16) return bad("the batch is too large: split it");
     if (seqs->n_seqs == 0 || seqs->total_q == 0) return ICUA_OK;
     int dev = 0;
-    if ((st = current(pages, k_out ? k_out : v_out, &dev)) != ICUA_OK) return st;
+    const bool scales = pages->dtype == ICUA_KV_Q8;
+    st = check_device_ptrs(&dev, {{pages->k, "the K pool"}, {k_out ? k_out : v_out, "the row array"}, {pages->v, "the V pool"},
+                                 {scales ? pages->k_scale : nullptr, "k_scale"}, {scales ? pages->v_scale : nullptr, "v_scale"},
+                                 {seqs->cu_q, "cu_q"}, {seqs->kv_len, "kv_len"}, {seqs->page_table, "page_table"}, {err_dev, "err_dev"},
+                                 {v_out, "v_out"}});
+    if (st != ICUA_OK) return st;
     p.k_out = k_out;
     p.v_out = v_out;
     p.err = err_dev;
@@ -374,7 +426,12 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
         return bad("scratch is null, not 16-byte aligned or smaller than icua_attn_paged_scratch_bytes");
     if (seqs->n_seqs == 0 || seqs->total_q == 0) return ICUA_OK;
     int dev = 0;
-    if ((st = current(pages, a->q, &dev)) != ICUA_OK) return st;
+    const bool scales = pages->dtype == ICUA_KV_Q8;
+    st = check_device_ptrs(&dev, {{pages->k, "the K pool"}, {a->q, "the row array"}, {pages->v, "the V pool"},
+                                 {scales ? pages->k_scale : nullptr, "k_scale"}, {scales ? pages->v_scale : nullptr, "v_scale"},
+                                 {seqs->cu_q, "cu_q"}, {seqs->kv_len, "kv_len"}, {seqs->page_table, "page_table"}, {err_dev, "err_dev"},
+                                 {a->out, "out"}, {a->scratch, "scratch"}});
+    if (st != ICUA_OK) return st;
     p.q = a->q;
     p.out = a->out;
     p.n_q = a->n_q;

@@ -1,9 +1,11 @@
 """GPU tests of calls of the paged K/V cache operators that the ordinary ones do not make: whole halves of a tile without
 a position, entries that contradict each other far back in a batch, hints and sizes at their ends."""
+import ctypes as C
+
 import pytest
 import torch
 
-from _paged import Cache, check_close
+from _paged import Cache, check_close, ptr
 from instantcua_b200 import _lib as L
 
 pytestmark = pytest.mark.gpu
@@ -210,4 +212,51 @@ def test_a_wait_that_gives_up_leaves_nan_rows_and_a_flag(n, kv, cache, typ):
     for out in (lost, silent):
         assert out[:n[0]].isnan().all() and torch.equal(out[n[0]:], want[n[0]:])
     c.err.zero_()
+    assert torch.equal(c.attend(q), want) and c.flags() == 0
+
+
+POINTERS = ["k", "v", "k_scale", "v_scale", "cu_q", "kv_len", "page_table", "err_dev"]
+
+
+@pytest.mark.parametrize("call,bad", [(c, b) for c, own in (("write", ["qkv", "q_out", "q_norm", "k_norm", "rope", "rope_rows"]),
+                                                            ("read", ["k_out", "v_out"]), ("attend", ["q", "out", "scratch"]))
+                                      for b in POINTERS + own])
+def test_every_pointer_to_host_memory_is_refused(call, bad):
+    """Each pointer of each call in pageable host memory: refused by name before anything is launched."""
+    c = Cache([2], [5], cache="q8").fill()
+    host = torch.zeros(1 << 18)
+    at = (host.data_ptr() + 255) // 256 * 256
+
+    def pick(name, t):
+        return at if name == bad else ptr(t)
+
+    pages = c.pages(**{x: at for x in POINTERS[:4] if x == bad})
+    seqs = c.seqs(**{x: at for x in POINTERS[4:7] if x == bad})
+    err, lib = pick("err_dev", c.err), L.lib()
+    rows, w, rope = c.randn(2, 8, 128), torch.ones(128, device="cuda"), torch.zeros(8, 64, 2, device="cuda")
+    idx, q, out = torch.zeros(2, dtype=torch.int32, device="cuda"), c.randn(2, 4, 128).half(), torch.zeros(2, 4, 128, device="cuda").half()
+    before = c.k.clone()
+    if call == "write":
+        r = L.IcuaKvRows(qkv=pick("qkv", rows), qkv_dtype=L.DT_F32, n_q=4, q_norm=pick("q_norm", w), k_norm=pick("k_norm", w), eps=1e-6,
+                         rope=pick("rope", rope), rope_rows=pick("rope_rows", idx), rope_len=8, q_out=pick("q_out", out), q_dtype=L.DT_F16)
+        status = lib.icua_kv_write(C.byref(pages), C.byref(seqs), C.byref(r), err, None)
+    elif call == "read":
+        kv = torch.zeros(2, 2, 128, device="cuda").half()
+        status = lib.icua_kv_read(C.byref(pages), C.byref(seqs), pick("k_out", kv), pick("v_out", kv), L.DT_F16, err, None)
+    else:
+        sc, need = c.scratch()
+        a = L.IcuaAttnPaged(q=pick("q", q), out=pick("out", out), dtype=L.DT_F16, n_q=4, scratch=pick("scratch", sc), scratch_bytes=need)
+        status = lib.icua_attn_paged(C.byref(pages), C.byref(seqs), C.byref(a), err, None)
+    assert status == L.ERR_INVALID
+    assert b"is not device memory" in lib.icua_global_error()
+    torch.cuda.synchronize()
+    assert torch.equal(c.k, before) and (out == 0).all()
+
+
+def test_lengths_and_tables_in_pinned_host_memory():
+    """The small arrays where the device reads them in place."""
+    c = Cache([3, 1], [40, 700], n_kv=2, n_q=8).fill()
+    q = c.randn(4, 8, 128).half()
+    want = c.attend(q).clone()
+    c.cu, c.kv_len, c.table = (x.cpu().pin_memory() for x in (c.cu, c.kv_len, c.table))
     assert torch.equal(c.attend(q), want) and c.flags() == 0
