@@ -434,7 +434,6 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
     if (st != ICUA_OK) return st;
     p.q = a->q;
     p.out = a->out;
-    p.n_q = a->n_q;
     p.group = a->n_q / pages->n_kv;
     p.max_rows = PA_ROWS_FEW;
     p.part = (float*)a->scratch;

@@ -58,7 +58,7 @@ struct PagedAttnParams {
     const void* q;
     void* out;
     long long q_stride, out_stride;
-    int n_q, group;
+    int group;
     float scale_log2;  // softmax scale x log2(e)
     int max_rows;      // sequences with more rows (n G) than this belong to another kernel,
     int alone;         //   or, when there is none in this call, break the caller's max_q (ERR_SEQ)
