@@ -137,23 +137,25 @@ icua_status check_cache(const icua_kv_pages* c, const icua_kv_seqs* s, PagesView
     return ICUA_OK;
 }
 
+// What a device is asked once (by whichever threads come first: they find the same).
 constexpr int MAX_DEVICES = 64;
 int sm_count(int dev) {
-    static int n[MAX_DEVICES];
-    if (dev < 0 || dev >= MAX_DEVICES) return 148;
-    if (n[dev] == 0) {
-        int v = 0;
-        n[dev] = cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0 ? v : 148;
-    }
-    return n[dev];
+    static std::atomic<int> known[MAX_DEVICES];
+    const bool in = dev >= 0 && dev < MAX_DEVICES;
+    int n = in ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (n > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    if (in) known[dev].store(n, std::memory_order_relaxed);
+    return n;
 }
 
 template <auto Kernel>
 cudaError_t allow_smem(int bytes, int dev) {
-    static bool done[MAX_DEVICES];
-    if (dev >= 0 && dev < MAX_DEVICES && done[dev]) return cudaSuccess;
+    static std::atomic<bool> done[MAX_DEVICES];
+    const bool in = dev >= 0 && dev < MAX_DEVICES;
+    if (in && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
     const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && dev >= 0 && dev < MAX_DEVICES) done[dev] = true;
+    if (e == cudaSuccess && in) done[dev].store(true, std::memory_order_release);
     return e;
 }
 

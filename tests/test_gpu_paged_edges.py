@@ -260,3 +260,33 @@ def test_lengths_and_tables_in_pinned_host_memory():
     want = c.attend(q).clone()
     c.cu, c.kv_len, c.table = (x.cpu().pin_memory() for x in (c.cu, c.kv_len, c.table))
     assert torch.equal(c.attend(q), want) and c.flags() == 0
+
+
+def test_calls_from_several_threads():
+    """Eight threads, a stream, a batch and a scratch each, all making their first calls together."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    caches, qs, wants = [], [], []
+    for i in range(8):
+        c = Cache([1 + 40 * (i % 2), 1], [300 + i, 5000 - 600 * i], n_kv=1 + i % 3, n_q=6, cache="q8" if i % 4 == 3 else F16).fill()
+        caches.append(c)
+        qs.append((c.randn(c.total, 6, 128) * 2).half())
+        wants.append(c.attend(qs[-1]).clone())
+    torch.cuda.synchronize()
+
+    def work(i):
+        st = torch.cuda.Stream()
+        bad = 0
+        with torch.cuda.stream(st):
+            sc = caches[i].scratch()
+            st.synchronize()
+            for _ in range(50):
+                out = caches[i].attend(qs[i], scratch=sc)
+                caches[i].read(F16)
+                st.synchronize()
+                bad += not torch.equal(out, wants[i])
+        return bad
+
+    with ThreadPoolExecutor(8) as pool:
+        assert list(pool.map(work, range(8))) == [0] * 8
+    assert all(c.flags() == 0 for c in caches)
