@@ -275,11 +275,15 @@ cudaError_t launch_attn_few(const PagedAttnParams& p, Share share, bool one_tile
 // 12.4, 32,768 36.6 / 30.1; with fewer heads the line, which always has every SM, catches up earlier.)
 constexpr int PA_ROWS_FEW = 32;
 constexpr int PA_CLUSTER_KEYS = 4096;
-// Up to PA_CTA_KEYS a CTA per item serves the others, without the line's counting and its join.  (Single tokens, 8
-// kv heads, bf16 / q8, in a graph, CTA against line: 20 sequences of 64 positions 4.6 / 5.6 against 8.8 / 10.6 us, of
-// 512 11.0 / 13.7 against 14.5 / 17.1, of 1,024 18.2 / 24.2 against 18.6 / 23.7; 256 of 1,024 165 / 144 against 173 /
-// 165.  Beyond, a batch of few items needs the line to fill the GPU, and one long sequence to be shared.)
+// Short ones of the others get a CTA per item, without the line's counting and its join: up to 256 positions, and 8 more
+// for each item up to PA_CTA_KEYS, since a batch of few items needs the line to fill the GPU.  (fp16 / q8, in a graph, CTA
+// against line.  28 rows: 1 item of 256 positions 9.0 / 8.1 against 10.0 / 10.1 us, of 512 12.9 / 11.8 against 10.1 / 10.1, of
+// 1,000 20.8 / 19.0 against 10.8 / 10.4; 24 items of 512 13.3 / 12.2 against 13.5 / 13.1, of 1,000 21.2 / 19.6 against 15.5 /
+// 13.5; 64 of 512 13.4 / 12.4 against 16.2 / 16.2, of 1,000 21.4 / 19.9 against 18.8 / 18.9; 128 of 1,000 21.6 / 20.4 against
+// 28.4 / 28.4.  8 rows: 24 of 512 9.5 / 9.5 against 10.3 / 10.9, of 1,000 16.0 / 16.0 against 11.0 / 11.6; 64 of 1,000 16.1 / 16.2
+// against 14.1 / 15.5; 128 of 1,000 16.2 / 16.5 against 17.2 / 18.5; 296 of 1,000 28.1 / 21.4 against 31.0 / 28.7.)
 constexpr int PA_CTA_KEYS = 1024;
+int cta_keys(int64_t items) { return (int)std::min<int64_t>(PA_CTA_KEYS, 256 + 8 * items); }
 static_assert(PA_ROWS_FEW <= 32, "the kernel's largest tile holds every item");
 
 // Tiles of the tensor-core kernel: a bound from what the host knows, and the shares of the keys that fill
@@ -474,8 +478,9 @@ icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs
     p.alone = !tc;
     if (e == cudaSuccess && !all_tc) {
         const bool one_tile = (int64_t)seqs->max_q * p.group <= 16;
-        const bool few = one_tile && (int64_t)seqs->n_seqs * pages->n_kv * PA_CLUSTER <= sm_count(dev);
-        const Share share = few && seqs->max_kv <= PA_CLUSTER_KEYS ? Share::cluster : seqs->max_kv <= PA_CTA_KEYS ? Share::cta : Share::line;
+        const int64_t items = (int64_t)seqs->n_seqs * pages->n_kv;
+        const bool few = one_tile && items * PA_CLUSTER <= sm_count(dev);
+        const Share share = few && seqs->max_kv <= PA_CLUSTER_KEYS ? Share::cluster : seqs->max_kv <= cta_keys(items) ? Share::cta : Share::line;
         if (share != Share::line) p.max_rows = one_tile ? 16 : 32;  // one tile per (sequence, kv head)
         e = q8 ? (f16 ? launch_attn_few<__half, true>(p, share, one_tile, tc_ran, dev, s)
                       : launch_attn_few<__nv_bfloat16, true>(p, share, one_tile, tc_ran, dev, s))

@@ -290,3 +290,17 @@ def test_calls_from_several_threads():
     with ThreadPoolExecutor(8) as pool:
         assert list(pool.map(work, range(8))) == [0] * 8
     assert all(c.flags() == 0 for c in caches)
+
+
+@pytest.mark.parametrize("cache,typ", TYPES, ids=name)
+@pytest.mark.parametrize("items", [(1, 1), (1, 2), (3, 8), (12, 8)], ids=str)
+def test_drafts_of_few_and_many_items_below_1024_positions(items, cache, typ):
+    """28 and 8 rows an item around the lengths where the work's split changes with the number of items."""
+    s, n_kv = items
+    for kv in (255, 257, 449, 1000, 1024):
+        for n, group in ((7, 4), (1, 8)):
+            c = Cache([n] * s, [max(n, kv - 13 * i) for i in range(s)], n_kv=n_kv, n_q=group * n_kv, cache=cache, typ=typ, seed=kv).fill()
+            q = (c.randn(c.total, c.n_q, 128) * 2).to(typ)
+            want, bound = c.attend64(q)
+            check_close(c.attend(q), want, bound, f"{kv} positions, {n} tokens")
+            assert c.flags() == 0
