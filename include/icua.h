@@ -325,15 +325,17 @@ icua_status icua_dequant(int32_t fmt, int32_t n_rows, int32_t k, const void* pac
  * allocated, copied or waited for, so they can be captured into a graph.  Lengths and page numbers
  * are read by the kernels, so a captured call follows what the arrays hold when it is replayed.
  * Arguments the host can see are checked before anything is launched, and pointers to be memory of the
- * current device (or managed memory; other than the pools and rows they may be pinned host memory, which
- * is read in place), not how far it reaches.  What only the device can see
- * is checked there: a page number outside [0, n_pages) is left out (not written, read as zeros, its
- * positions masked) and sets ICUA_FLAG_PAGE; a sequence whose entries contradict each other (cu_q
- * that descends or passes total_q, a length below 0 or above max_pages * page_size) counts as
- * without tokens, a token without a position or a rotation row is left out, and both set
- * ICUA_FLAG_SEQ.  ICUA_FLAG_WAIT: a bounded wait inside icua_attn_paged gave up; the rows it was for
- * are NaN.  err_dev: optional device int32 that the flags are OR-ed into; without it left-out tokens
- * show by their rows alone. */
+ * current device (or managed memory; other than the pools and rows they may be pinned host memory,
+ * which is read in place), not how far it reaches.  What only the device can see is checked there, and
+ * tells by flags that are OR-ed into err_dev (an optional device int32):
+ *   ICUA_FLAG_PAGE  a page number outside [0, n_pages): not written, read as zeros, its positions masked;
+ *   ICUA_FLAG_SEQ   a sequence whose entries contradict each other (cu_q that descends or passes total_q,
+ *                   a length below 0 or above max_pages * page_size): it counts as without tokens, its
+ *                   rows stay as they were.  In icua_kv_write and icua_kv_read also a token without a
+ *                   position (kv_len < n) or, in the first, without a rotation row: not written, read as
+ *                   zeros (icua_attn_paged gives such a token zeros and sets nothing).  In
+ *                   icua_attn_paged also a sequence with more than max_q tokens, where it is left out;
+ *   ICUA_FLAG_WAIT  a bounded wait inside icua_attn_paged gave up: the rows it was for are NaN. */
 enum { ICUA_DT_F32 = 0, ICUA_DT_BF16 = 1, ICUA_DT_F16 = 2 }; /* row types, as icua_gemv's x_dtype */
 /* Third cache type: int8 codes with one fp32 scale per row (position, head): scale = max|x| / 127,
  * code = x / scale to the nearest (2^-15 of a step around a tie may go either way); a row of zeros has
@@ -345,10 +347,10 @@ enum { ICUA_FLAG_WAIT = 4, ICUA_FLAG_PAGE = 16, ICUA_FLAG_SEQ = 32 };
 
 /* The cache.  Row (page, head, r) is row page * page_rows + head * head_rows + r of both pools, r <
  * page_size; page_rows = head_rows = 0 means dense pages [page][head][r] (page_rows = n_kv *
- * page_size, head_rows = page_size).  Other strides (multiples of 16) lay pages over a cache that
- * exists: an engine-style [head][max_context][128] cache is pages of page_rows = page_size and
- * head_rows = max_context.  16-bit rows are 256 bytes in the engine's cache order (16-byte chunk c
- * of position p at place c ^ (p & 7)), q8 rows 128 codes in plain order. */
+ * page_size, head_rows = page_size).  Other strides (multiples of 16) lay pages over a cache of the
+ * caller's that exists: [head][max_context][128] is pages of page_rows = page_size and head_rows =
+ * max_context (the caches of an engine's sessions are not handed out).  16-bit rows are 256 bytes, 16-byte
+ * chunk c of position p at place c ^ (p & 7), q8 rows 128 codes in plain order. */
 typedef struct icua_kv_pages {
     void* k;            /* pools of rows */
     void* v;

@@ -28,7 +28,7 @@
 //
 // Measured on a B200 (6.54 TB/s by copy): 48 single tokens over 3 .. 16,000 positions, 32:8 heads, bf16, 76 us =
 // 5.5 TB/s; 64 over about 2,000 positions, 16:8 heads, q8, 72 us = 3.8 TB/s, bound by the conversions (half of
-// the issue slots at three warps per scheduler); 24 drafts of 7 tokens, 32:8 heads, fp16, 54 us = 3.6 TB/s, bound
+// the issue slots at three warps per scheduler); 24 drafts of 7 tokens, 32:8 heads, fp16, 56 us = 3.5 TB/s, bound
 // by latency (the two tiles' registers leave two warps per scheduler); one token over 4,096 positions, 16:8
 // heads, bf16, in a cluster per kv head 10.3 us against 12.3 us dealt as a line and joined.
 #pragma once

@@ -19,10 +19,10 @@
 // Bound: the chain of one half's block (softmax about 1,950 clocks, then P V and the next scores 1,150), of
 // which two run against each other: about 3,200 clocks per 256 x 128 scores, where the exponentials (16 per
 // clock and SM) and the products (64 clocks per M128 N128 K16 step) take 2,048 each.  Measured on a B200 (1,629
-// TFLOP/s by library GEMM): a prompt of 8,192 tokens, 32:8 heads, bf16, in 0.536 ms = 1,025 TFLOP/s; a chunk of
-// 500 over 8,001 positions, 16:8 heads, q8, 84 us, there bound by the four converting warps (1,800 clocks per
-// 128 rows) and by the factors' shared-memory reads.  Tried and slower: part of the exponentials as polynomials
-// on the FMA pipe (560 against 549 us), two threads per row (575), rows as matrix fragments (608).
+// TFLOP/s by library GEMM): a prompt of 8,192 tokens, 32:8 heads, bf16, in 0.544 ms = 1,010 TFLOP/s; a chunk of
+// 500 over 8,001 positions, 16:8 heads, fp16 51 us, q8 86 us (74 from L2), there bound by the four converting warps
+// (1,800 clocks per 128 rows) and by the factors' shared-memory reads.  Tried and slower: part of the exponentials as
+// polynomials on the FMA pipe (560 against 549 us), two threads per row (575), rows as matrix fragments (608).
 // Every wait is bounded: one that gives up raises ERR_WAIT_PREFILL, the half's rows become NaN, and the CTA still
 // drains its copies and products and frees its tensor memory.
 #pragma once
