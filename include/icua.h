@@ -422,8 +422,8 @@ uint64_t icua_attn_paged_scratch_bytes(const icua_kv_pages* pages, const icua_kv
  * prompts, together in one call.  Scores, softmax and sums in fp32, probabilities rounded to the
  * type of q.  In a q8 cache a probability is rounded after it was multiplied by its key's V scale, relative to
  * the largest such product: all products are held as precisely down to 2^-14 (fp16) or 2^-126 (bf16) of it,
- * smaller ones are off by up to 2^-25 of it in fp16; the sums take them unrounded.  A V scale below 1e-30
- * counts as 1e-30.  Rows of a 16-bit cache behind a sequence's end are never used; rows of its own new
+ * smaller ones are off by up to 2^-25 of it in fp16; the sums take them unrounded.  A product below 2^-126
+ * of the largest is left out, of the sums too.  A V scale below 1e-30 counts as 1e-30.  Rows of a 16-bit cache behind a sequence's end are never used; rows of its own new
  * tokens must be finite, since a later token's infinity or NaN reaches the earlier ones of the same
  * call (0 x inf).  A token without a position (kv_len < n) gets zeros. */
 icua_status icua_attn_paged(const icua_kv_pages* pages, const icua_kv_seqs* seqs, const icua_attn_paged_args* args,
