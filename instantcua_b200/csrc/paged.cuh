@@ -200,8 +200,9 @@ __device__ __forceinline__ void store4(T* p, const float* x) {
 // A half-warp per head vector: lane l holds elements 4 l .. 4 l + 3 and 64 + 4 l .., the two halves of four
 // rotation pairs.  y = x rsqrt(mean x^2 + eps) w, then (y_j c - y_{j+64} s, y_{j+64} c + y_j s), in fp32; q rows
 // are rounded to the output type, k and v rows to the cache type or to int8 codes: scale = max|x| / 127 in fp32
-// and code = x / scale to the nearest even, so a code is off by at most half a step.  A row that holds a NaN
-// or an infinity gets the scale NaN and reads back as NaN throughout.  A row of zeros gets the scale 1 (K) or KV_ZERO_V.
+// and code = x / scale to the nearest, so a code is off by at most half a step (and 2^-15 of one, by the reciprocal
+// that x is multiplied with).  A row that holds a NaN or an infinity gets the scale NaN and reads back as NaN
+// throughout.  A row of zeros gets the scale 1 (K) or KV_ZERO_V.
 // A CTA takes TOK tokens: a warp each looks its sequence, position and page up, then every token's vectors
 // are dealt to 16 / TOK half-warps, each with its token's rotation row and the norm weights in registers and
 // four vectors' loads in flight.  Bound: HBM for many tokens (each row is read once and written once; TOK = 4
